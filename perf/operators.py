@@ -206,7 +206,7 @@ def prepare(case, seed):
             min_p = torch.where(pick % 5 == 0, 0.02 + 0.1 * r(), min_p)
             temp = torch.where(pick % 8 == 7, 0.0, temp)
         s.update(logits=lg.to(DT[case["dt"]])[:, :v], temp=temp, top_k=top_k.to(torch.int32), top_p=top_p, min_p=min_p, u=r(),
-                 out=torch.zeros(rows, **i32), space=None)
+                 out=torch.zeros(rows, **i32))
     return s
 
 
@@ -221,7 +221,7 @@ def _desc(s):
     if "desc" not in s:
         kg, _ = _be()
         pool = s["pool"]
-        s["desc"] = kg.kg_pool(pool[:, 0].data_ptr(), pool[:, 1].data_ptr(), pool.shape[0], pool.shape[2], pool.shape[3], pool.shape[4],
+        s["desc"] = kg.page_pool(pool[:, 0].data_ptr(), pool[:, 1].data_ptr(), pool.shape[0], pool.shape[2], pool.shape[3], pool.shape[4],
                                s["case"]["dt"], page_stride=pool.stride(0), row_stride=pool.stride(2), head_stride=pool.stride(3))
     return s["desc"]
 
@@ -308,11 +308,8 @@ def _sample(s):
     lg = s["logits"]
     if own:
         _, be = _be()
-        if s["space"] is None:
-            s["space"] = torch.empty(max(be.sample_logits_bytes(lg.shape[0], lg.shape[1]), 1), dtype=torch.uint8, device=lg.device)
         be.sample_logits_dev(lg.shape[0], lg.shape[1], c["dt"], lg.data_ptr(), lg.stride(0), s["temp"].data_ptr(), s["top_k"].data_ptr(),
-                             s["top_p"].data_ptr(), s["min_p"].data_ptr(), s["u"].data_ptr(), s["out"].data_ptr(), s["space"].data_ptr(),
-                             s["space"].numel(), _stream())
+                             s["top_p"].data_ptr(), s["min_p"].data_ptr(), s["u"].data_ptr(), s["out"].data_ptr(), _stream())
         return s["out"]
     v = lg.shape[1]
     x, at = torch.sort(lg.double(), dim=-1, descending=True, stable=True)  # ties: the lowest index first
