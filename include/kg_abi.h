@@ -95,7 +95,8 @@ void kg_config_micro(kg_config *c);
  * rotation) bit-identically to TurboQuantKVCache::new. */
 int kg_ctx_create(const kg_config *cfg, int device, kg_ctx **out);
 void kg_ctx_destroy(kg_ctx *ctx);
-/* Last error message of this context ("" if none). */
+/* Last error message of this context ("" if none). NULL: the message of the
+ * calling thread's last kg_pool_* or kg_sample_logits_dev call without a context. */
 const char *kg_last_error(const kg_ctx *ctx);
 const char *kg_status_string(int status);
 /* InferenceBackend::device_name */
@@ -220,6 +221,137 @@ int kg_verify_dev(kg_ctx *ctx, int32_t n_seq, const int32_t *seq_ids, const int3
 /* Host-pointer form; synchronises. */
 int kg_verify(kg_ctx *ctx, int32_t n_seq, const int32_t *seq_ids, const int32_t *start_pos, const int32_t *tokens,
               const int32_t *drafts, int32_t k, const float *draft_probs, int32_t *accepted, int32_t *n_accepted);
+
+/* ---- serving operators over a caller-owned page pool ----
+ * One step of a server that batches requests of unlike lengths, with every
+ * length on the device: kg_pool_plan_dev turns request lengths into block
+ * tables, slot maps and row offsets, kg_pool_store_dev writes the new K/V rows
+ * into their pages, kg_pool_attend_dev attends the new rows over the pages
+ * (a prompt chunk, a draft path or a single token, in one ragged batch), and
+ * kg_sample_logits_dev draws the next tokens. The reference's batch path runs
+ * its sequences one by one on the host (src/transformer.rs:3588-3606) and its
+ * PagedKVCache (crates/katgpt-transformer/src/kv_cache.rs:187-420) is host
+ * state; the kg_paged_* calls below keep that cache inside a context, these
+ * keep nothing: pool, tables and workspace are the caller's device memory.
+ *
+ * All pointers are device pointers unless said otherwise, the work is enqueued
+ * on `stream` (a stream of the context's device; NULL = the legacy default
+ * stream), nothing is allocated and nothing synchronises, so every call can be
+ * captured into a CUDA graph after one eager call. The caller's current device
+ * is left as it was. Host-side argument checks come first and return
+ * KG_ERR_INVALID_ARG or KG_ERR_UNSUPPORTED with a message in kg_last_error
+ * (for a NULL context, kg_last_error(NULL) has the calling thread's). Device-
+ * side checks (a table entry or slot outside the pool, lengths that do not fit)
+ * skip the access and set a word that kg_pool_status reports. Calls of one
+ * context on different streams may overlap on the device as long as their
+ * outputs and workspaces are distinct; the host-side calls themselves are
+ * serialised by the caller, as for every call on a context. */
+
+typedef enum { KG_DT_F32 = 0, KG_DT_BF16 = 1, KG_DT_F16 = 2 } kg_dtype;
+
+/* A pool of K/V pages. Row t of page p, K/V head h starts at
+ * k + p * page_stride + t * row_stride + h * head_stride (elements; the same
+ * strides for v), head_dim contiguous elements. The framework's own page layout
+ * [page][K page_size x kv_dim | V page_size x kv_dim] has page_stride
+ * 2 * page_size * kv_dim, row_stride kv_dim, head_stride head_dim and
+ * v = k + page_size * kv_dim. Bases 16-byte aligned, strides multiples of 8. */
+typedef struct {
+    void *k;
+    void *v;
+    int64_t page_stride;
+    int64_t row_stride;
+    int64_t head_stride;
+    int32_t n_pages;
+    int32_t page_size;  /* positions per page: 16, 32, 64 or 128; n_pages * page_size < 2^31 */
+    int32_t n_kv_head;
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t dtype;      /* KG_DT_BF16 or KG_DT_F16 */
+} kg_pool;
+
+/* Block tables and slot maps of one step. Request r holds cached_len[r]
+ * positions in the pages table[r][0 .. ceil(cached_len[r] / page_size)) and adds
+ * new_len[r] (0 allowed). In request order every request takes the pages that
+ * its new positions still need from the tail of free_pages[0 .. *n_free) (the
+ * last entry first, as PagedKVCache's free list) into table[r][...]; the rest of
+ * the table is left as it was. table is [n_req][table_width].
+ * Written: *n_free_out = what is left (may be n_free itself), cu_q[n_req + 1] =
+ * running sum of new_len, kv_len[r] = cached_len[r] + new_len[r], and for each
+ * new token t < cu_q[n_req], in request order: slots[t] = page * page_size + row
+ * of its K/V, req_of[t], positions[t]; entries from cu_q[n_req] to max_tokens
+ * are -1 (padding). *status is KG_OK, or KG_ERR_OOM (too few free pages) or
+ * KG_ERR_INVALID_ARG (a negative length, more than max_tokens new tokens, a
+ * request wider than the table or longer than 2^31 - 1, *n_free outside [0,
+ * n_pages], a page used here outside the pool); then nothing is taken: tables
+ * and the free count stay, cu_q and kv_len are all 0 and the token entries all
+ * -1, so that the calls that follow in the step do nothing. At most 16384
+ * requests. Buffers must not overlap, except n_free_out = n_free. */
+int kg_pool_plan_dev(kg_ctx *ctx, int32_t page_size, int32_t n_pages, int32_t n_req, const int32_t *cached_len,
+                     const int32_t *new_len, int32_t *table, int32_t table_width, const int32_t *free_pages,
+                     const int32_t *n_free, int32_t *n_free_out, int32_t max_tokens, int32_t *cu_q, int32_t *kv_len,
+                     int32_t *slots, int32_t *req_of, int32_t *positions, int32_t *status, void *stream);
+
+/* Rows of new K and V into their slots: row i of k and v (src_dtype, KV head h
+ * at i * row_stride + h * head_stride elements, head_dim contiguous) is rounded
+ * to the pool's type (nearest even) and written at page slots[i] / page_size,
+ * row slots[i] % page_size. Negative slots (padding) are skipped, slots past the
+ * pool are skipped and reported. Distinct rows have distinct slots; of two rows
+ * with one slot either may win, element by element. Rows 16-byte aligned:
+ * bases, and strides in multiples of 16 bytes. */
+int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const int32_t *slots, int32_t src_dtype,
+                      const void *k, const void *v, int64_t row_stride, int64_t head_stride, void *stream);
+
+/* Attention of new rows over the pages. Request r owns the rows
+ * cu_q[r] .. cu_q[r + 1) of q and out; its last row stands at position
+ * kv_len[r] - 1, the others before it, and with `causal` row i attends the
+ * positions up to its own, otherwise all kv_len[r] of them (as forward_prefill
+ * does over its prompt). Query head h reads KV head h / (n_head / n_kv_head):
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]
+ * with f32 scores, statistics and sums; a row that attends nothing (kv_len 0,
+ * or a row before position 0) becomes zeros. The probabilities enter the second
+ * product in the pool's type, everything is rounded once at the end. q and out
+ * have the pool's type, out row i head h at i * out_row_stride + h *
+ * out_head_stride; q and out must not overlap. Rows outside every request's
+ * range are left as they were. Page contents past kv_len are never used; those
+ * before it are finite. Device-side checks: cu_q non-decreasing within [0,
+ * total_q], kv_len within [0, table_width * page_size], or the request's rows
+ * are left as they were; a table entry outside the pool reads as zeros; either
+ * is reported. n_head at most 64 times n_kv_head, at most 16384 requests.
+ * workspace: kg_pool_attend_bytes() bytes, 16-byte aligned, for partial results
+ * when one request's positions are split over several CTAs; its content need
+ * not be kept or initialised, and calls that may overlap on the device (other
+ * streams, two graphs) need one each. kg_pool_attend_bytes returns a negative
+ * kg_status for arguments that kg_pool_attend_dev refuses. */
+int64_t kg_pool_attend_bytes(const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q);
+int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q,
+                       const int32_t *cu_q, const int32_t *kv_len, const int32_t *table, int32_t table_width,
+                       const void *q, int64_t q_row_stride, int64_t q_head_stride, void *out, int64_t out_row_stride,
+                       int64_t out_head_stride, float scale, int32_t causal, void *workspace, int64_t workspace_bytes,
+                       void *stream);
+
+/* Next tokens from logits, with every row's own parameters and given uniform
+ * numbers (kg_sample_dev draws from probabilities with the slot's generator).
+ * Row i of logits (dtype, vocab entries, ld elements apart) is ordered by value,
+ * ties by the lower index; with w_j = exp((x_j - max) / temperature[i]):
+ *   top_k[i] > 0: the first top_k[i] tokens stay;
+ *   top_p[i] < 1: of those, the shortest prefix whose w reaches top_p[i] of
+ *                 their sum stays (at least one token);
+ *   min_p[i] > 0: of all, those with w_j >= min(min_p[i], 1) stay;
+ * tokens_out[i] = the first index, in index order, whose running sum of the
+ * remaining w exceeds u[i] times their total (u in [0, 1); below reads as 0,
+ * 1 and above as the last). temperature[i] <= 0 or NaN: the largest logit.
+ * -inf and NaN logits are never drawn; several +inf share the draw; a row with
+ * no token left by those rules gives -1. Sums are exact integer sums of w in
+ * units of 2^-44, so a result does not depend on the order of the sums.
+ * temperature, top_k, top_p, min_p: [n_rows] each, NULL = 1, off, off, off.
+ * vocab at most 262144. Any alignment of logits that fits the type. */
+int kg_sample_logits_dev(kg_ctx *ctx, int32_t n_rows, int32_t vocab, int32_t dtype, const void *logits, int64_t ld,
+                         const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                         const float *u, int32_t *tokens_out, void *stream);
+
+/* Waits for the context's device and returns what the device-side checks of the
+ * calls above saw since the last kg_pool_status: KG_OK, KG_ERR_INVALID_ARG or
+ * KG_ERR_TIMEOUT. Not during a stream capture. */
+int kg_pool_status(kg_ctx *ctx);
 
 /* ---- multi-GPU sequence shards (one context per GPU) ----
  * Sequences shard across GPUs with replicated weights; the one exchange is an

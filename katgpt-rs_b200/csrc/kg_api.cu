@@ -15,6 +15,7 @@
 
 #include "kg_bf16.cuh"
 #include "kg_internal.h"
+#include "kg_serve.h"
 
 namespace kg {
 void host_normals(uint64_t seed, int64_t n, float *out);
@@ -141,7 +142,7 @@ const char *kg_status_string(int s) {
     }
 }
 
-const char *kg_last_error(const kg_ctx *ctx) { return ctx ? ctx->err.c_str() : "null context"; }
+const char *kg_last_error(const kg_ctx *ctx) { return ctx ? ctx->err.c_str() : kg::serve::thread_error().c_str(); }
 const char *kg_device_name(const kg_ctx *ctx) { return ctx ? ctx->dev_name.c_str() : "CUDA"; }
 int64_t kg_weights_count(const kg_config *cfg) { return cfg ? kg::weights_count(*cfg) : -1; }
 int64_t kg_tq_packed_len(int64_t dim, int32_t bits) { return packed_len(dim, bits); }
@@ -233,7 +234,9 @@ int kg_ctx_create(const kg_config *cfg, int device, kg_ctx **out) {
     if ((rc = dalloc(ctx, &ctx->codes, rows * (ctx->kpl + ctx->vpl)))) return bail(rc);
     if ((rc = dalloc(ctx, &ctx->norms, rows * 2))) return bail(rc);
     if ((rc = dalloc(ctx, &ctx->util, rows))) return bail(rc);
-    if ((rc = dalloc(ctx, &ctx->d_err, 1))) return bail(rc);
+    if ((rc = dalloc(ctx, &ctx->d_err, 1)) || (rc = dalloc(ctx, &ctx->serve_err, 1))) return bail(rc);
+    e = cudaMemset(ctx->serve_err, 0, sizeof(int));
+    if (e != cudaSuccess) return bail(cuda_fail(ctx, e, "context init"));
     e = kg::sampler_init(ctx);
     if (e != cudaSuccess) return bail(cuda_fail(ctx, e, "sampler init"));
 

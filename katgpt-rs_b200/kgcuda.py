@@ -52,6 +52,27 @@ class KgSqParams(ctypes.Structure):
 
 SQ_LEVELS = 64
 
+KG_DT_F32, KG_DT_BF16, KG_DT_F16 = 0, 1, 2
+DTYPES = {"f32": KG_DT_F32, "bf16": KG_DT_BF16, "f16": KG_DT_F16}
+
+
+class KgPool(ctypes.Structure):
+    """Mirror of kg_pool (include/kg_abi.h): a caller-owned pool of K/V pages."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("n_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+def page_pool(k_ptr, v_ptr, n_pages, page_size, n_kv_head, head_dim, dtype="bf16", page_stride=None, row_stride=None,
+              head_stride=None):
+    """A kg_pool over device memory (raw addresses, strides in elements). Without
+    strides: rows of n_kv_head * head_dim, a page's K rows then its V rows."""
+    kvd = n_kv_head * head_dim
+    return KgPool(k_ptr, v_ptr, 2 * page_size * kvd if page_stride is None else page_stride,
+                  kvd if row_stride is None else row_stride, head_dim if head_stride is None else head_stride, n_pages,
+                  page_size, n_kv_head, head_dim, DTYPES[dtype])
+
 
 class KgError(RuntimeError):
     def __init__(self, status, msg):
@@ -111,6 +132,13 @@ def lib():
             "kg_sample_dev": (ctypes.c_int, [P, I32, P, P, I64, P, P]),
             "kg_sample": (ctypes.c_int, [P, I32, P, P, P]),
             "kg_verify_dev": (ctypes.c_int, [P, I32, P, P, P, P, I32, P, P, P, P]),
+            "kg_pool_plan_dev": (ctypes.c_int, [P, I32, I32, I32, P, P, P, I32, P, P, P, I32, P, P, P, P, P, P, P]),
+            "kg_pool_store_dev": (ctypes.c_int, [P, ctypes.POINTER(KgPool), I32, P, I32, P, P, I64, I64, P]),
+            "kg_pool_attend_bytes": (I64, [ctypes.POINTER(KgPool), I32, I32, I32]),
+            "kg_pool_attend_dev": (ctypes.c_int, [P, ctypes.POINTER(KgPool), I32, I32, I32, P, P, P, I32, P, I64, I64, P, I64,
+                                                  I64, F32, I32, P, I64, P]),
+            "kg_sample_logits_dev": (ctypes.c_int, [P, I32, I32, I32, P, I64, P, P, P, P, P, P, P]),
+            "kg_pool_status": (ctypes.c_int, [P]),
             "kg_forward_prefill": (ctypes.c_int, [P, I32, P, P, I32, P]),
             "kg_forward_prefill_dev": (ctypes.c_int, [P, I32, P, P, I32, P, P]),
             "kg_verify": (ctypes.c_int, [P, I32, P, P, P, P, I32, P, P, P]),
@@ -405,6 +433,46 @@ class CudaBackend:
         self._check(lib().kg_verify(self._h, n, _ptr(ids), _ptr(start_pos), _ptr(tokens), _ptr(drafts), k, _ptr(q),
                                     _ptr(acc), _ptr(cnt)))
         return acc, cnt
+
+    # ---- serving operators over a caller-owned page pool (device pointers as integers)
+    def pool_plan_dev(self, page_size, n_pages, n_req, cached_ptr, new_ptr, table_ptr, table_width, free_ptr, n_free_ptr,
+                      n_free_out_ptr, max_tokens, cu_q_ptr, kv_len_ptr, slots_ptr, req_of_ptr, positions_ptr, status_ptr,
+                      stream_ptr=None):
+        """Block tables, slot maps and row offsets of a step from request lengths (kg_pool_plan_dev)."""
+        self._check(lib().kg_pool_plan_dev(self._h, page_size, n_pages, n_req, cached_ptr, new_ptr, table_ptr, table_width,
+                                           free_ptr, n_free_ptr, n_free_out_ptr, max_tokens, cu_q_ptr, kv_len_ptr,
+                                           slots_ptr, req_of_ptr, positions_ptr, status_ptr, stream_ptr))
+
+    def pool_store_dev(self, pool, n_rows, slots_ptr, src_dtype, k_ptr, v_ptr, row_stride, head_stride, stream_ptr=None):
+        """New K/V rows into the slots of a page_pool (kg_pool_store_dev); src_dtype "f32", "bf16" or "f16"."""
+        self._check(lib().kg_pool_store_dev(self._h, pool, n_rows, slots_ptr, DTYPES[src_dtype], k_ptr, v_ptr, row_stride,
+                                            head_stride, stream_ptr))
+
+    @staticmethod
+    def pool_attend_bytes(pool, n_req, n_head, total_q):
+        """Workspace bytes of pool_attend_dev (kg_pool_attend_bytes)."""
+        n = lib().kg_pool_attend_bytes(pool, n_req, n_head, total_q)
+        if n < 0:
+            raise KgError(int(n), lib().kg_last_error(None).decode())
+        return int(n)
+
+    def pool_attend_dev(self, pool, n_req, n_head, total_q, cu_q_ptr, kv_len_ptr, table_ptr, table_width, q_ptr,
+                        q_row_stride, q_head_stride, out_ptr, out_row_stride, out_head_stride, scale, causal, workspace_ptr,
+                        workspace_bytes, stream_ptr=None):
+        """Attention of new rows over the pages of a page_pool (kg_pool_attend_dev)."""
+        self._check(lib().kg_pool_attend_dev(self._h, pool, n_req, n_head, total_q, cu_q_ptr, kv_len_ptr, table_ptr,
+                                             table_width, q_ptr, q_row_stride, q_head_stride, out_ptr, out_row_stride,
+                                             out_head_stride, scale, causal, workspace_ptr, workspace_bytes, stream_ptr))
+
+    def sample_logits_dev(self, n_rows, vocab, dtype, logits_ptr, ld, temperature_ptr, top_k_ptr, top_p_ptr, min_p_ptr,
+                          u_ptr, tokens_ptr, stream_ptr=None):
+        """Next tokens from logits with top-k, top-p and min-p (kg_sample_logits_dev)."""
+        self._check(lib().kg_sample_logits_dev(self._h, n_rows, vocab, DTYPES[dtype], logits_ptr, ld, temperature_ptr,
+                                               top_k_ptr, top_p_ptr, min_p_ptr, u_ptr, tokens_ptr, stream_ptr))
+
+    def pool_status(self):
+        """Waits for the device; raises what the device-side checks of these calls saw (kg_pool_status)."""
+        self._check(lib().kg_pool_status(self._h))
 
     # ---- multi-GPU sequence shards
     def comm_init(self, uid, world, rank):
