@@ -1,96 +1,453 @@
 // kg_pool_attn.cu — kg_pool_attend_dev: attention of new rows over a paged K/V
 // pool, ragged over requests.
+//
+// One pass over the positions with a running maximum m and sum l per row:
+//   o = sum_j 2^(s_j - m) v_j,  l = sum_j 2^(s_j - m),  s_j = scale log2(e) q.k_j
+// A part of the positions gives (o, m, l); parts of one item join as
+//   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
+// The work is one line of units cut into equal parts (kg_pool_sched.h), so that
+// one long sequence fills the device as well as many short ones, and the lengths
+// are read on the device.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstring>
+
+#include "kg_dev.cuh"
 #include "kg_pdl.cuh"
+#include "kg_pool_attn.cuh"
 #include "kg_serve.h"
 
 namespace kg {
 namespace serve {
 namespace {
 
-struct AttendArgs {
-    kg_pool p;
-    int n_req, n_head, group, total_q, width, causal;
-    const int32_t *cu, *kv, *table;
-    const void *q;
-    void *out;
-    int64_t q_row, q_head, o_row, o_head;
-    float scale;
-    int *err;
+using namespace as;
+
+// ---------------------------------------------------------------------------
+// Short requests (at most 64 rows: single tokens, draft paths) on mma.sync:
+// rows (token, query head of the group) x positions. Bound by the bytes of K and
+// V; a producer warp keeps a ring of 64-position stages filled by TMA, one box
+// per page, and four warps split a stage by rows (groups of 16) and by positions.
+// Each keeps its own running maximum and sum, joined at the end of the item.
+constexpr int SHORT_THREADS = 160, SHORT_LEAST = 2;
+
+template <int D>
+struct ShortCfg {
+    static constexpr int HALF_BYTES = kShortUnit * 128;              // 64 positions x 64 elements
+    static constexpr int OP_BYTES = HALF_BYTES * (D / 64);           // K or V of a stage
+    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int SCRATCH = 4 * 16 * 36 * 4;
+    static constexpr int SMEM = 1024 + STAGES * 2 * OP_BYTES + SCRATCH + 4 * 16 * 2 * 4 + 2 * STAGES * 8 + 16;
 };
 
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ KvMaps maps, const AttendArgs a) {
+    using C = ShortCfg<D>;
+    extern __shared__ __align__(1024) uint8_t raw[];
+    uint8_t *sm = raw + ((1024u - (sa(raw) & 1023u)) & 1023u);
+    float *scratch = reinterpret_cast<float *>(sm + C::STAGES * 2 * C::OP_BYTES);  // [4 warps][16 rows][36]
+    float2 *stat = reinterpret_cast<float2 *>(scratch + 4 * 16 * 36);              // [4 warps][16 rows] (max, sum)
+    uint64_t *full = reinterpret_cast<uint64_t *>(stat + 4 * 16), *empty = full + C::STAGES;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + C::STAGES);
+    __shared__ long long part_sm[SHORT_THREADS / 32 + 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 4);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    pdl_wait();
+    int req;
+    long long off, units;
+    find_part<SHORT_THREADS, false>(a, c, gridDim.x, SHORT_LEAST, part_sm, req, off, units);  // (synchronises)
+    if (threadIdx.x < 2) a.meta[2 * c + threadIdx.x].x = 0;
+    __syncthreads();
+    if (units == 0) return;
+    Walk<false> w;
+    w.start(a, req, off, units);
+
+    if (warp == 4) {  // producer: lane i loads box i of a unit
+        const int rows = min(a.page_size, kShortUnit), pages = kShortUnit / rows, boxes = pages * (D / 64) * 2;
+        const int piece = lane % pages, half = lane / pages % (D / 64), which = lane / (pages * (D / 64));
+        const CUtensorMap *tm = which ? &maps.v : &maps.k;
+        const int dst = which * C::OP_BYTES + half * C::HALF_BYTES + piece * rows * 128;
+        int it = 0;
+        do {
+            for (int u = 0; u < w.n; ++u, ++it) {
+                const int s = it % C::STAGES, pos = (w.p.unit + u) * kShortUnit + piece * rows;
+                int page = a.n_pages;  // outside the pool: the box becomes zeros
+                if (lane < boxes && pos < w.kv) {
+                    const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
+                    if (e >= 0 && e < a.n_pages) page = e;
+                    else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+                }
+                int ok = 1;
+                if (lane == 0) {
+                    ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, a.err);
+                    if (ok) mbar_expect_tx(&full[s], 2 * C::OP_BYTES);
+                }
+                if (!__shfl_sync(~0u, ok, 0)) {
+                    drain_loads(full, C::STAGES, it);
+                    return;
+                }
+                if (lane < boxes)
+                    tma_load_4d(sm + s * 2 * C::OP_BYTES + dst, tm, half * 64, w.p.head, pos % a.page_size, page, &full[s]);
+            }
+        } while (w.next(a));
+        return;
+    }
+
+    const int gid = lane >> 2, tig = lane & 3;
+    int it = 0;
+    do {
+        const int rows = w.q * a.s.group, wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;  // row groups
+        const int rg = warp % wm, pg = warp / wm;
+        // Q fragments of rows 16 rg + gid and + 8
+        uint32_t qf[D / 16][4];
+        int lim[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = rg * 16 + gid + 8 * i, t = row / a.s.group, h = w.p.head * a.s.group + row % a.s.group;
+            const bool in = row < rows;
+            lim[i] = in ? row_limit(a.s, w.q, w.kv, t) : 0;
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.q) + (w.q0 + t) * a.q_row + h * a.q_head);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                qf[k][i] = in ? __ldg(src + k * 8 + tig) : 0u;
+                qf[k][i + 2] = in ? __ldg(src + k * 8 + tig + 4) : 0u;
+            }
+        }
+        float o[D / 8][4];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int u = 0; u < w.n; ++u, ++it) {
+            const int s = it % C::STAGES;
+            // (a wait that gave up skips the work, not the barriers below)
+            const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, a.err);
+            uint8_t *st = sm + s * 2 * C::OP_BYTES;
+            bool wrote = false;
+            for (int b = 0; ok && b < wm; ++b) {
+                const int p0 = (pg * wm + b) * 16, pos0 = (w.p.unit + u) * kShortUnit + p0;
+                if (pos0 >= w.kv) break;
+                if (pos0 + 16 > w.kv) {  // rows behind the last position: whatever the page holds must not reach the sums
+                    for (int i = lane; i < 16 * (D / 8); i += 32) {
+                        const int r = i / (D / 8), ch = i % (D / 8);
+                        if (pos0 + r >= w.kv)
+                            *reinterpret_cast<uint4 *>(st + C::OP_BYTES + (ch >> 3) * C::HALF_BYTES + (p0 + r) * 128 + (ch & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                    }
+                    wrote = true;
+                    __syncwarp();
+                }
+                float sc[2][4] = {};
+                {
+                    const int r = p0 + (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
+                    const uint32_t base = sa(st) + r * 128;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int ch = k * 2 + cb;
+                        uint32_t kf[4];
+                        ldsm4(base + (ch >> 3) * C::HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4), kf);
+                        mma16816<T>(sc[0], qf[k], kf[0], kf[1]);
+                        mma16816<T>(sc[1], qf[k], kf[2], kf[3]);
+                    }
+                }
+                uint32_t pf[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float x[4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            x[n * 2 + e] = pos0 + n * 8 + tig * 2 + e < lim[i] ? sc[n][i * 2 + e] * a.scale : -INFINITY;
+                    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                    const float mn = fmaxf(m[i], mx);
+                    if (__any_sync(~0u, mn != m[i])) {
+                        const float f = mn == -INFINITY ? 1.0f : exp2_approx(m[i] - mn);
+                        l[i] *= f;
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) {
+                            o[n][i * 2] *= f;
+                            o[n][i * 2 + 1] *= f;
+                        }
+                        m[i] = mn;
+                    }
+                    const float base = mn == -INFINITY ? 0.0f : mn;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e] - base);
+                    l[i] += (x[0] + x[1]) + (x[2] + x[3]);
+                    pf[i] = Cvt<T>::pack(x[0], x[1]);
+                    pf[i + 2] = Cvt<T>::pack(x[2], x[3]);
+                }
+                {
+                    const int r = p0 + (lane & 7) + (((lane >> 3) & 1) << 3), cb = lane >> 4;
+                    const uint32_t base = sa(st) + C::OP_BYTES + r * 128;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int ch = k * 2 + cb;
+                        uint32_t vf[4];
+                        ldsm4t(base + (ch >> 3) * C::HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4), vf);
+                        mma16816<T>(o[2 * k], pf, vf[0], vf[1]);
+                        mma16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+                    }
+                }
+            }
+            if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the stage again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        // join the warps that share rows and write the item
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(~0u, l[i], 1);
+            l[i] += __shfl_xor_sync(~0u, l[i], 2);
+            if (tig == 0) stat[warp * 16 + gid + 8 * i] = make_float2(m[i], l[i]);
+        }
+        bar_consumers();
+        auto top_of = [&](int g, int r) {
+            float x = -INFINITY;
+            for (int k = g; k < 4; k += wm) x = fmaxf(x, stat[k * 16 + r].x);
+            return x;
+        };
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f[i] = m[i] == -INFINITY ? 0.0f : exp2_approx(m[i] - top_of(rg, gid + 8 * i));
+        const bool whole = w.whole();
+        const int slot = 2 * c + w.slot();
+        float *part = a.part + slot * a.slot_floats;
+        for (int d0 = 0; d0 < D; d0 += 32) {
+            float *mine = scratch + warp * 16 * 36;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                if (n / 4 == d0 / 32)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<float2 *>(mine + (gid + 8 * i) * 36 + (n & 3) * 8 + tig * 2) =
+                            make_float2(o[n][i * 2] * f[i], o[n][i * 2 + 1] * f[i]);
+            bar_consumers();
+            for (int i = threadIdx.x; i < rows * 8; i += 128) {
+                const int row = i >> 3, d = (i & 7) * 4, g = row >> 4, r = row & 15;
+                float4 sum = make_float4(0, 0, 0, 0);
+                for (int k = g; k < 4; k += wm) {
+                    const float4 x = *reinterpret_cast<const float4 *>(scratch + (k * 16 + r) * 36 + d);
+                    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+                }
+                const float top = top_of(g, r);
+                float total = 0.0f;
+                for (int k = g; k < 4; k += wm) {
+                    const float2 x = stat[k * 16 + r];
+                    if (x.x != -INFINITY) total += x.y * exp2_approx(x.x - top);
+                }
+                if (whole) {
+                    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+                    T *dst = static_cast<T *>(a.out) + (w.q0 + row / a.s.group) * a.o_row +
+                             (w.p.head * a.s.group + row % a.s.group) * a.o_head + d0 + d;
+                    *reinterpret_cast<uint2 *>(dst) =
+                        make_uint2(Cvt<T>::pack(sum.x * inv, sum.y * inv), Cvt<T>::pack(sum.z * inv, sum.w * inv));
+                } else {
+                    *reinterpret_cast<float4 *>(part + (int64_t)row * D + d0 + d) = sum;
+                    if (d0 == 0 && d == 0) reinterpret_cast<float2 *>(part + (int64_t)a.rows * D)[row] = make_float2(top, total);
+                }
+            }
+            bar_consumers();
+        }
+        if (!whole && threadIdx.x == 0) a.meta[slot] = make_int4(w.ends() ? 3 : 1, w.r, w.p.head, 0);
+    } while (w.next(a));
+}
+
+// Joins the parts of an item that was cut: CTA c looks after the item that
+// begins in part c and ends beyond it. Part sums are added in the order of the
+// parts, so results do not depend on timing.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, int parts) {
+    pdl_wait();
+    __shared__ int s_last;
+    __shared__ float4 sums[8][32];
+    __shared__ float2 stat[8];
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int4 me = a.meta[2 * c + 1];
+    if (me.x == 0) return;
+    if (threadIdx.x == 0) {
+        int e = c + 1;
+        while (e < parts - 1 && a.meta[2 * e].x == 1) ++e;
+        s_last = e;
+    }
+    __syncthreads();
+    int q0, q, kv;
+    req_len(a, me.y, q0, q, kv);
+    const int rows = q * a.s.group, n = s_last - c + 1;
+    auto slot = [&](int i) { return a.part + (i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.slot_floats; };
+    constexpr int PER = D / 32;  // dims of a lane
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        auto stat_of = [&](int i) { return reinterpret_cast<const float2 *>(slot(i) + (int64_t)a.rows * D)[row]; };
+        float top = -INFINITY;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, stat_of(i).x);
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        float o[PER] = {}, l = 0.0f;
+#pragma unroll 4
+        for (int i = warp; i < n; i += 8) {
+            const float2 s = stat_of(i);
+            const float f = s.x == -INFINITY ? 0.0f : exp2_approx(s.x - top);
+            const float *p = slot(i) + (int64_t)row * D + lane * PER;
+            l += s.y * f;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] += p[e] * f;
+        }
+        sums[warp][lane] = make_float4(o[0], o[1], PER > 2 ? o[PER - 2] : 0.0f, PER > 2 ? o[PER - 1] : 0.0f);
+        if (lane == 0) stat[warp] = make_float2(0.0f, l);
+        __syncthreads();
+        if (warp == 0) {
+            float4 t = make_float4(0, 0, 0, 0);
+            float total = 0.0f;
+            for (int k = 0; k < 8; ++k) {
+                const float4 x = sums[k][lane];
+                t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+                total += stat[k].y;
+            }
+            const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+            T *dst = static_cast<T *>(a.out) + (q0 + row / a.s.group) * a.o_row + (me.z * a.s.group + row % a.s.group) * a.o_head + lane * PER;
+            reinterpret_cast<uint32_t *>(dst)[0] = Cvt<T>::pack(t.x * inv, t.y * inv);
+            if (PER > 2) reinterpret_cast<uint32_t *>(dst)[1] = Cvt<T>::pack(t.z * inv, t.w * inv);
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Long requests, one warp per (row, query head).
 template <typename T>
 __device__ __forceinline__ float to_f(T x);
 template <>
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <>
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
 
-// Whether request r's lengths can be used (reported otherwise).
-__device__ __forceinline__ bool request_ok(const AttendArgs &a, int r) {
-    const int q0 = a.cu[r], q1 = a.cu[r + 1], kv = a.kv[r];
-    return q0 >= 0 && q1 >= q0 && q1 <= a.total_q && kv >= 0 && kv <= (int64_t)a.width * a.p.page_size;
-}
-
-// One warp per (row, query head): a running maximum and sum over the row's
-// positions, one position at a time.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_rows_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(128) attend_rows_kernel(AttendArgs a, kg_pool p) {
     pdl_wait();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, n_head = a.s.group * a.s.n_kv;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int row = (int)(w / a.n_head), h = (int)(w % a.n_head);
+    const int row = (int)(w / n_head), h = (int)(w % n_head);
     if (row >= a.total_q) return;
     int r = -1;
-    for (int i = lane; i < a.n_req; i += 32)
-        if (request_ok(a, i)) {
-            if (row >= a.cu[i] && row < a.cu[i + 1]) r = i;
-        } else {
-            atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
-        }
+    for (int i = lane; i < a.n_req; i += 32) {
+        int q0, q, kv;
+        if (req_len(a, i, q0, q, kv) && row >= q0 && row < q0 + q) r = i;
+    }
     for (int d = 16; d; d >>= 1) r = max(r, __shfl_xor_sync(~0u, r, d));
     if (r < 0) return;
-    const int kv = a.kv[r], at = kv - a.cu[r + 1] + row, n = a.causal ? min(at + 1, kv) : kv;
+    int q0, q, kv;
+    req_len(a, r, q0, q, kv);
+    if (is_short(a.s, q)) return;
+    const int n = row_limit(a.s, q, kv, row - q0);
     constexpr int E = D / 32;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_row + h * a.q_head + lane * E;
-    const int hk = h / a.group;
+    const T *qp = static_cast<const T *>(a.q) + row * a.q_row + h * a.q_head + lane * E;
+    const int hk = h / a.s.group;
     float qf[E], o[E], m = -INFINITY, l = 0.0f;
     for (int e = 0; e < E; ++e) {
-        qf[e] = to_f(q[e]) * a.scale;
+        qf[e] = to_f(qp[e]) * a.scale;
         o[e] = 0.0f;
     }
     for (int j = 0; j < n; ++j) {
-        const int page = a.table[(int64_t)r * a.width + j / a.p.page_size];
-        const bool ok = page >= 0 && page < a.p.n_pages;
+        const int page = a.table[(int64_t)r * a.width + j / a.page_size];
+        const bool ok = page >= 0 && page < a.n_pages;
         if (!ok) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
-        const int64_t off = ok ? page * a.p.page_stride + (j % a.p.page_size) * a.p.row_stride + hk * a.p.head_stride + lane * E : 0;
+        const int64_t off = ok ? page * p.page_stride + (j % a.page_size) * p.row_stride + hk * p.head_stride + lane * E : 0;
         float s = 0.0f;
-        for (int e = 0; e < E; ++e) s += ok ? qf[e] * to_f(static_cast<const T *>(a.p.k)[off + e]) : 0.0f;
+        for (int e = 0; e < E; ++e) s += ok ? qf[e] * to_f(static_cast<const T *>(p.k)[off + e]) : 0.0f;
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-        const float mn = fmaxf(m, s), c = __expf(m - mn), p = __expf(s - mn);
-        l = l * c + p;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + (ok ? p * to_f(static_cast<const T *>(a.p.v)[off + e]) : 0.0f);
+        const float mn = fmaxf(m, s), c = exp2f(m - mn), pr = exp2f(s - mn);
+        l = l * c + pr;
+        for (int e = 0; e < E; ++e) o[e] = o[e] * c + (ok ? pr * to_f(static_cast<const T *>(p.v)[off + e]) : 0.0f);
         m = mn;
     }
     T *out = static_cast<T *>(a.out) + row * a.o_row + h * a.o_head + lane * E;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    for (int e = 0; e < E; ++e) out[e] = from_f<T>(o[e] * inv);
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = Cvt<T>::pack(o[e] * inv, o[e + 1] * inv);
 }
 
-template <typename T>
-cudaError_t launch(const AttendArgs &a, cudaStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)a.total_q * a.n_head + 3) / 4));
-    if (a.p.head_dim == 64) return launch_pdl(attend_rows_kernel<T, 64>, grid, dim3(128), 0, s, a);
-    return launch_pdl(attend_rows_kernel<T, 128>, grid, dim3(128), 0, s, a);
+// ---------------------------------------------------------------------------
+// Host
+
+// The pool as [pages][page rows][heads][head_dim], boxes of one page's rows (64
+// at most), one head and 64 elements (128 bytes, the swizzle's width).
+bool pool_map(CUtensorMap *m, const kg_pool &p, const void *base) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_kv_head, (cuuint64_t)p.page_size, (cuuint64_t)p.n_pages};
+    auto bytes = [&](int64_t stride, int64_t count) { return (cuuint64_t)(count > 1 ? stride : p.head_dim) * 2; };
+    const cuuint64_t strides[3] = {bytes(p.head_stride, p.n_kv_head), bytes(p.row_stride, p.page_size), bytes(p.page_stride, p.n_pages)};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(p.page_size, kShortUnit), 1}, es[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Workspace: [meta][part sums]
+struct Space {
+    int rows;
+    int64_t slot_floats, bytes;
+};
+Space space_of(const kg_pool &p, int n_head, int total_q) {
+    Space s;
+    const int64_t rows = (int64_t)total_q * (n_head / p.n_kv_head);
+    s.rows = (int)std::min<int64_t>((rows + 15) / 16 * 16, kShortRows);
+    s.slot_floats = (int64_t)s.rows * (p.head_dim + 2);
+    s.bytes = 2 * kMaxParts * ((int64_t)sizeof(int4) + s.slot_floats * 4);
+    return s;
+}
+
+template <typename T, int D>
+cudaError_t launch(const kg_pool &p, AttendArgs a, cudaStream_t s) {
+    KvMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    if (!pool_map(&maps.k, p, p.k) || !pool_map(&maps.v, p, p.v)) return cudaErrorInvalidValue;
+    using C = ShortCfg<D>;
+    cudaError_t e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
+    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a);
+    if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D>, dim3(parts, std::min(a.rows, 16)), dim3(256), 0, s, a, parts);
+    if (e == cudaSuccess && (int64_t)a.total_q * a.s.group > kShortRows) {
+        const dim3 grid((unsigned)(((int64_t)a.total_q * a.s.group * a.s.n_kv + 3) / 4));
+        e = launch_pdl(attend_rows_kernel<T, D>, grid, dim3(128), 0, s, a, p);
+    }
+    return e;
 }
 
 int check(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q) {
@@ -112,7 +469,7 @@ extern "C" {
 
 int64_t kg_pool_attend_bytes(const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q) {
     if (int rc = kg::serve::check(nullptr, pool, n_req, n_head, total_q)) return rc;
-    return 16;
+    return kg::serve::space_of(*pool, n_head, total_q).bytes;
 }
 
 int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q,
@@ -124,6 +481,7 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
     if (int rc = check(ctx, pool, n_req, n_head, total_q)) return rc;
     if (table_width < 1) return fail(ctx, KG_ERR_INVALID_ARG, "attend: table_width must be positive");
     const bool some = n_req > 0 && total_q > 0;
+    const Space sp = space_of(*pool, n_head, total_q);
     if (some) {
         if (!cu_q || !kv_len || !table || !q || !out || !workspace) return fail(ctx, KG_ERR_INVALID_ARG, "attend: null pointer");
         if (q == out) return fail(ctx, KG_ERR_INVALID_ARG, "attend: q and out must not overlap");
@@ -134,18 +492,39 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
             !nested(pool->head_dim, {q_row_stride, total_q}, {q_head_stride, n_head}, {0, 1}) ||
             !nested(pool->head_dim, {out_row_stride, total_q}, {out_head_stride, n_head}, {0, 1}))
             return fail(ctx, KG_ERR_INVALID_ARG, "attend: rows overlap at these strides");
-        if (workspace_bytes < kg_pool_attend_bytes(pool, n_req, n_head, total_q))
-            return fail(ctx, KG_ERR_INVALID_ARG, "attend: workspace smaller than kg_pool_attend_bytes");
-        if (!(scale > -INFINITY && scale < INFINITY)) return fail(ctx, KG_ERR_INVALID_ARG, "attend: scale must be finite");
+        if (workspace_bytes < sp.bytes) return fail(ctx, KG_ERR_INVALID_ARG, "attend: workspace smaller than kg_pool_attend_bytes");
+        if (!(scale >= 0.0f && scale < INFINITY)) return fail(ctx, KG_ERR_INVALID_ARG, "attend: scale must be finite and not negative");
     }
     if (!ctx) return fail(ctx, KG_ERR_INVALID_ARG, "null context");
     if (!some) return KG_OK;
     DeviceGuard dg(ctx->device);
     if (dg.err != cudaSuccess) return cuda_fail(ctx, dg.err, "kg_pool_attend_dev");
-    AttendArgs a{*pool, n_req, n_head, n_head / pool->n_kv_head, total_q, table_width, causal, cu_q, kv_len, table, q, out,
-                 q_row_stride, q_head_stride, out_row_stride, out_head_stride, scale, ctx->serve_err};
+    AttendArgs a;
+    a.s = Shape{n_head / pool->n_kv_head, pool->n_kv_head, 2 * (128 / (n_head / pool->n_kv_head)), causal != 0};
+    a.n_req = n_req;
+    a.total_q = total_q;
+    a.width = table_width;
+    a.page_size = pool->page_size;
+    a.n_pages = pool->n_pages;
+    a.cu = cu_q;
+    a.kv = kv_len;
+    a.table = table;
+    a.q = q;
+    a.out = out;
+    a.q_row = q_row_stride;
+    a.q_head = q_head_stride;
+    a.o_row = out_row_stride;
+    a.o_head = out_head_stride;
+    a.scale = scale * 1.4426950408889634f;
+    a.err = ctx->serve_err;
+    a.meta = static_cast<int4 *>(workspace);
+    a.part = reinterpret_cast<float *>(a.meta + 2 * kMaxParts);
+    a.slot_floats = sp.slot_floats;
+    a.rows = sp.rows;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = pool->dtype == KG_DT_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+    const bool bf = pool->dtype == KG_DT_BF16;
+    const cudaError_t e = pool->head_dim == 64 ? (bf ? launch<__nv_bfloat16, 64>(*pool, a, s) : launch<__half, 64>(*pool, a, s))
+                                               : (bf ? launch<__nv_bfloat16, 128>(*pool, a, s) : launch<__half, 128>(*pool, a, s));
     return e == cudaSuccess ? KG_OK : cuda_fail(ctx, e, "kg_pool_attend_dev");
 }
 

@@ -1,0 +1,185 @@
+// kg_pool_attn.cuh — what the two kernels of kg_pool_attend_dev share: their
+// arguments, the walk over a CTA's part of the line of units, and the partial
+// results that the joining kernel reads.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "kg_async.cuh"
+#include "kg_pool_sched.h"
+
+namespace kg {
+namespace serve {
+
+constexpr int kMaxParts = 512;  // CTAs of one kernel's line (3 per SM of a B200 at most)
+
+struct AttendArgs {
+    Shape s;
+    int n_req, total_q, width, page_size, n_pages;
+    const int32_t *cu, *kv, *table;
+    const void *q;
+    void *out;
+    int64_t q_row, q_head, o_row, o_head;
+    float scale;  // times log2(e)
+    int *err;
+    // partial results: slot 2 c of CTA c for the item its part begins inside, slot 2 c + 1 for the one it
+    // ends inside without having begun in; `rows` rows of head_dim sums, then rows of (max, sum)
+    float *part;
+    int64_t slot_floats;
+    int rows;
+    int4 *meta;  // per slot: {0 unused, 1 used, 3 used and the item's end, request, head, tile}
+};
+struct KvMaps {
+    CUtensorMap k, v;
+};
+
+template <typename T>
+struct Cvt;
+template <>
+struct Cvt<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+template <>
+struct Cvt<__half> {
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A producer that gave up on a wait: its loads in flight end before the block's shared memory is given back (each wait
+// bounded again). `it` loads were issued into a ring of `stages`.
+__device__ __forceinline__ void drain_loads(uint64_t *full, int stages, int it) {
+    for (int i = it > stages ? it - stages : 0; i < it; ++i) {
+        const long long t0 = clock64();
+        while (!as::mbar_try(&full[i % stages], (i / stages) & 1) && clock64() - t0 < (1ll << 28)) {
+        }
+    }
+}
+
+// 4-D tiled load: one page's rows of one head, 64 elements wide
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *tm, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];\n" ::"r"(as::sa(dst)),
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(w), "r"(as::sa(bar))
+        : "memory");
+}
+
+// lengths of request r, zeros where they cannot be used
+__device__ __forceinline__ bool req_len(const AttendArgs &a, int r, int &q0, int &q, int &kv) {
+    q0 = a.cu[r];
+    const int q1 = a.cu[r + 1];
+    kv = a.kv[r];
+    const bool ok = lengths_ok(q0, q1, kv, a.total_q, min((int64_t)a.width * a.page_size, (int64_t)kMaxKv));
+    q = ok ? q1 - q0 : 0;
+    if (!ok) kv = 0;
+    return ok;
+}
+
+// This CTA's part: where it begins and how many units it has. At most `parts`
+// parts of at least `least` units. Every thread of the block calls it (NT
+// threads); `sm` holds NT / 32 + 2 numbers.
+template <int NT, bool LONG>
+__device__ void find_part(const AttendArgs &a, int c, int parts, int least, long long *sm, int &req, long long &off,
+                          long long &units) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.n_req + NT - 1) / NT, r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) {
+        int q0, q, kv;
+        if (!req_len(a, r, q0, q, kv) && c == 0) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+        mine += request_units(a.s, LONG, q, kv);
+    }
+    long long incl = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long u = __shfl_up_sync(~0u, incl, d);
+        if (lane >= d) incl += u;
+    }
+    if (lane == 31) sm[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += sm[w];
+        total += sm[w];
+    }
+    parts = (int)min((long long)parts, (total + least - 1) / least);
+    const long long b = c < parts ? part_begin(total, c, parts) : 0, e = c < parts ? part_begin(total, c + 1, parts) : 0;
+    units = e - b;
+    if (units > 0 && before <= b && b < before + mine) {
+        long long at = before;
+        for (int r = r0; r < r1; ++r) {
+            int q0, q, kv;
+            req_len(a, r, q0, q, kv);
+            const long long n = request_units(a.s, LONG, q, kv);
+            if (b < at + n) {
+                sm[NT / 32] = r;
+                sm[NT / 32 + 1] = b - at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    req = units > 0 ? (int)sm[NT / 32] : 0;
+    off = units > 0 ? sm[NT / 32 + 1] : 0;
+}
+
+// The items of a part, in order.
+template <bool LONG>
+struct Walk {
+    int r, q0, q, kv;
+    Place p;
+    int n;           // units of the item here
+    long long left;  // units after it
+    __device__ __forceinline__ void start(const AttendArgs &a, int req, long long off, long long units) {
+        r = req;
+        left = units;
+        if (units <= 0) return;
+        req_len(a, r, q0, q, kv);
+        p = place_of(a.s, LONG, q, kv, off);
+        take();
+    }
+    __device__ __forceinline__ void take() {
+        n = (int)min(left, (long long)(p.units - p.unit));
+        left -= n;
+    }
+    // to the next item; false at the end
+    __device__ __forceinline__ bool next(const AttendArgs &a) {
+        if (left <= 0) return false;
+        p.unit = 0;
+        if (LONG && p.tile + 1 < long_tiles(a.s, q)) {
+            ++p.tile;
+        } else {
+            p.tile = 0;
+            if (++p.head == a.s.n_kv) {
+                p.head = 0;
+                do {
+                    ++r;
+                    req_len(a, r, q0, q, kv);
+                } while (request_units(a.s, LONG, q, kv) == 0);
+            }
+        }
+        p.units = LONG ? long_units(a.s, q, kv, p.tile) : short_units(a.s, q, kv);
+        take();
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return p.unit == 0 && n == p.units; }
+    // slot of a partial item: 0 when its first units are another CTA's
+    __device__ __forceinline__ int slot() const { return p.unit == 0 ? 1 : 0; }
+    __device__ __forceinline__ bool ends() const { return p.unit + n == p.units; }
+};
+
+}  // namespace serve
+}  // namespace kg

@@ -1,0 +1,96 @@
+// kg_pool_sched.h — how kg_pool_attend_dev's work is cut: plain integer
+// arithmetic, used by the kernels and, compiled as C++, by a CPU test.
+//
+// A request whose rows (new tokens x query heads per K/V head) fit kShortRows
+// is "short": one item per K/V head, units of kShortUnit positions. The others
+// are "long": one item per (K/V head, tile of tokens), units of kLongUnit
+// positions up to the tile's last attended one. An item always has a unit, so
+// that rows which attend nothing get their zeros. The units of all items in
+// order (request, head, tile, unit) form one line that is cut into equal parts,
+// one per CTA: a part is a run of units that may begin and end inside an item.
+#pragma once
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define KG_HD __host__ __device__ __forceinline__
+#else
+#define KG_HD inline
+#endif
+
+namespace kg {
+namespace serve {
+
+constexpr int kShortRows = 64, kShortUnit = 64, kLongUnit = 128;
+constexpr int kMaxKv = 2147483647 - 256;  // a unit that begins before the last position ends inside 31 bits
+
+struct Shape {
+    int group;      // query heads per K/V head
+    int n_kv;       // K/V heads
+    int tile;       // tokens of a long item
+    int causal;
+};
+
+KG_HD bool lengths_ok(int q0, int q1, int kv, int total_q, int64_t room) {
+    return q0 >= 0 && q1 >= q0 && q1 <= total_q && kv >= 0 && kv <= room;
+}
+KG_HD bool is_short(const Shape &s, int q) { return (int64_t)q * s.group <= kShortRows; }
+
+// units of one head's item of a short request (0: none)
+KG_HD int short_units(const Shape &s, int q, int kv) {
+    if (q == 0 || !is_short(s, q)) return 0;
+    return kv > 0 ? (kv - 1) / kShortUnit + 1 : 1;
+}
+KG_HD int long_tiles(const Shape &s, int q) { return q == 0 || is_short(s, q) ? 0 : (q - 1) / s.tile + 1; }
+// positions that token t's row attends: [0, limit)
+KG_HD int row_limit(const Shape &s, int q, int kv, int t) {
+    if (!s.causal) return kv;
+    const int64_t n = (int64_t)kv - q + t + 1;
+    return n < 0 ? 0 : (int)n;
+}
+KG_HD int long_units(const Shape &s, int q, int kv, int i) {
+    const int64_t end = (int64_t)(i + 1) * s.tile;
+    const int n = row_limit(s, q, kv, (int)(end < q ? end : q) - 1);
+    return n > 0 ? (n - 1) / kLongUnit + 1 : 1;
+}
+KG_HD int64_t long_units_of_head(const Shape &s, int q, int kv) {
+    const int n = long_tiles(s, q);
+    int64_t sum = 0;
+    for (int i = 0; i < n; ++i) sum += long_units(s, q, kv, i);
+    return sum;
+}
+// units of a whole request in the line of short or of long items
+KG_HD int64_t request_units(const Shape &s, bool is_long, int q, int kv) {
+    return (is_long ? long_units_of_head(s, q, kv) : short_units(s, q, kv)) * s.n_kv;
+}
+// the first unit of part c of `parts`
+KG_HD int64_t part_begin(int64_t units, int c, int parts) { return units / parts * c + units % parts * c / parts; }
+
+// A place in the line: item (head, tile) of a request, its first unit here and its length.
+struct Place {
+    int head, tile, unit, units;
+};
+KG_HD Place place_of(const Shape &s, bool is_long, int q, int kv, int64_t off) {
+    Place p;
+    if (!is_long) {
+        p.units = short_units(s, q, kv);
+        p.head = (int)(off / p.units);
+        p.unit = (int)(off % p.units);
+        p.tile = 0;
+        return p;
+    }
+    const int64_t per = long_units_of_head(s, q, kv);
+    p.head = (int)(off / per);
+    int64_t rest = off % per;
+    p.tile = 0;
+    while (true) {
+        p.units = long_units(s, q, kv, p.tile);
+        if (rest < p.units) break;
+        rest -= p.units;
+        ++p.tile;
+    }
+    p.unit = (int)rest;
+    return p;
+}
+
+}  // namespace serve
+}  // namespace kg

@@ -130,6 +130,7 @@ def test_plan_refusals(kg, kw, code, text):
     (dict(wsb=0), INVALID, "workspace"),
     (dict(scale=float("inf")), INVALID, "scale"),
     (dict(scale=float("nan")), INVALID, "scale"),
+    (dict(scale=-0.125), INVALID, "scale"),
     (dict(), INVALID, "null context"),
     (dict(qrs=64, qhs=64 * 12, ors=64, ohs=64 * 12), INVALID, "null context"),  # head-major
     (dict(n_req=0, cu=None, kv=None, table=None, q=None, out=None, ws=None), INVALID, "null context"),

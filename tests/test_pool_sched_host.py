@@ -1,0 +1,14 @@
+"""The cut of kg_pool_attend_dev's work (katgpt-rs_b200/csrc/kg_pool_sched.h, the kernels' own source) on the CPU."""
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_every_unit_belongs_to_one_part(tmp_path):
+    exe = tmp_path / "pool_sched_host"
+    r = subprocess.run(["g++", "-O1", "-std=c++17", os.path.join(ROOT, "tests", "host", "pool_sched_host.cpp"), "-o", str(exe)],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout
