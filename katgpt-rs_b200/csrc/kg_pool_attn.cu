@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <type_traits>
 
 #include "kg_dev.cuh"
 #include "kg_pdl.cuh"
@@ -293,12 +294,12 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
 // Joins the parts of an item that was cut: CTA c looks after the item that
 // begins in part c and ends beyond it. Part sums are added in the order of the
 // parts, so results do not depend on timing.
-template <typename T, int D>
+template <typename T, int D, bool LONG>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, int parts) {
     pdl_wait();
     __shared__ int s_last;
     __shared__ float4 sums[8][32];
-    __shared__ float2 stat[8];
+    __shared__ float part_l[8];
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int4 me = a.meta[2 * c + 1];
     if (me.x == 0) return;
@@ -310,26 +311,31 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, in
     __syncthreads();
     int q0, q, kv;
     req_len(a, me.y, q0, q, kv);
-    const int rows = q * a.s.group, n = s_last - c + 1;
+    const int n = s_last - c + 1, group = a.s.group, tq = a.s.tile / 2;
+    const int rows = LONG ? 256 : q * group;
     auto slot = [&](int i) { return a.part + (i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.slot_floats; };
     constexpr int PER = D / 32;  // dims of a lane
     for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-        auto stat_of = [&](int i) { return reinterpret_cast<const float2 *>(slot(i) + (int64_t)a.rows * D)[row]; };
+        const int i = LONG ? row & 127 : row;
+        const int tok = LONG ? (me.w * 2 + (row >> 7)) * tq + i / group : i / group;
+        if (LONG && (i >= tq * group || tok >= q)) continue;
+        auto stat_of = [&](int k) { return reinterpret_cast<const float2 *>(slot(k) + (int64_t)a.rows * D)[row]; };
         float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, stat_of(i).x);
+        for (int k = lane; k < n; k += 32) top = fmaxf(top, stat_of(k).x);
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
         float o[PER] = {}, l = 0.0f;
 #pragma unroll 4
-        for (int i = warp; i < n; i += 8) {
-            const float2 s = stat_of(i);
-            const float f = s.x == -INFINITY ? 0.0f : exp2_approx(s.x - top);
-            const float *p = slot(i) + (int64_t)row * D + lane * PER;
+        for (int k = warp; k < n; k += 8) {
+            const float2 s = stat_of(k);
+            if (s.x == -INFINITY) continue;  // nothing was attended there, nothing was written
+            const float f = exp2_approx(s.x - top);
+            const float *p = slot(k) + (int64_t)row * D + lane * PER;
             l += s.y * f;
 #pragma unroll
             for (int e = 0; e < PER; ++e) o[e] += p[e] * f;
         }
         sums[warp][lane] = make_float4(o[0], o[1], PER > 2 ? o[PER - 2] : 0.0f, PER > 2 ? o[PER - 1] : 0.0f);
-        if (lane == 0) stat[warp] = make_float2(0.0f, l);
+        if (lane == 0) part_l[warp] = l;
         __syncthreads();
         if (warp == 0) {
             float4 t = make_float4(0, 0, 0, 0);
@@ -337,68 +343,15 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, in
             for (int k = 0; k < 8; ++k) {
                 const float4 x = sums[k][lane];
                 t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
-                total += stat[k].y;
+                total += part_l[k];
             }
             const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-            T *dst = static_cast<T *>(a.out) + (q0 + row / a.s.group) * a.o_row + (me.z * a.s.group + row % a.s.group) * a.o_head + lane * PER;
+            T *dst = static_cast<T *>(a.out) + (int64_t)(q0 + tok) * a.o_row + (me.z * group + i % group) * a.o_head + lane * PER;
             reinterpret_cast<uint32_t *>(dst)[0] = Cvt<T>::pack(t.x * inv, t.y * inv);
             if (PER > 2) reinterpret_cast<uint32_t *>(dst)[1] = Cvt<T>::pack(t.z * inv, t.w * inv);
         }
         __syncthreads();
     }
-}
-
-// ---------------------------------------------------------------------------
-// Long requests, one warp per (row, query head).
-template <typename T>
-__device__ __forceinline__ float to_f(T x);
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_rows_kernel(AttendArgs a, kg_pool p) {
-    pdl_wait();
-    const int lane = threadIdx.x & 31, n_head = a.s.group * a.s.n_kv;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int row = (int)(w / n_head), h = (int)(w % n_head);
-    if (row >= a.total_q) return;
-    int r = -1;
-    for (int i = lane; i < a.n_req; i += 32) {
-        int q0, q, kv;
-        if (req_len(a, i, q0, q, kv) && row >= q0 && row < q0 + q) r = i;
-    }
-    for (int d = 16; d; d >>= 1) r = max(r, __shfl_xor_sync(~0u, r, d));
-    if (r < 0) return;
-    int q0, q, kv;
-    req_len(a, r, q0, q, kv);
-    if (is_short(a.s, q)) return;
-    const int n = row_limit(a.s, q, kv, row - q0);
-    constexpr int E = D / 32;
-    const T *qp = static_cast<const T *>(a.q) + row * a.q_row + h * a.q_head + lane * E;
-    const int hk = h / a.s.group;
-    float qf[E], o[E], m = -INFINITY, l = 0.0f;
-    for (int e = 0; e < E; ++e) {
-        qf[e] = to_f(qp[e]) * a.scale;
-        o[e] = 0.0f;
-    }
-    for (int j = 0; j < n; ++j) {
-        const int page = a.table[(int64_t)r * a.width + j / a.page_size];
-        const bool ok = page >= 0 && page < a.n_pages;
-        if (!ok) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
-        const int64_t off = ok ? page * p.page_stride + (j % a.page_size) * p.row_stride + hk * p.head_stride + lane * E : 0;
-        float s = 0.0f;
-        for (int e = 0; e < E; ++e) s += ok ? qf[e] * to_f(static_cast<const T *>(p.k)[off + e]) : 0.0f;
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-        const float mn = fmaxf(m, s), c = exp2f(m - mn), pr = exp2f(s - mn);
-        l = l * c + pr;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + (ok ? pr * to_f(static_cast<const T *>(p.v)[off + e]) : 0.0f);
-        m = mn;
-    }
-    T *out = static_cast<T *>(a.out) + row * a.o_row + h * a.o_head + lane * E;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = Cvt<T>::pack(o[e] * inv, o[e + 1] * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -418,22 +371,27 @@ bool pool_map(CUtensorMap *m, const kg_pool &p, const void *base) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Workspace: [meta][part sums]
+// Workspace: [meta][part sums], for the short requests' kernel and then, where
+// the rows of a call could make a request long, for the long requests'.
 struct Space {
     int rows;
-    int64_t slot_floats, bytes;
+    bool may_long;
+    int64_t slot_floats, long_at, long_floats, bytes;
 };
 Space space_of(const kg_pool &p, int n_head, int total_q) {
     Space s;
     const int64_t rows = (int64_t)total_q * (n_head / p.n_kv_head);
     s.rows = (int)std::min<int64_t>((rows + 15) / 16 * 16, kShortRows);
     s.slot_floats = (int64_t)s.rows * (p.head_dim + 2);
-    s.bytes = 2 * kMaxParts * ((int64_t)sizeof(int4) + s.slot_floats * 4);
+    s.may_long = rows > kShortRows;
+    s.long_at = 2 * kMaxParts * ((int64_t)sizeof(int4) + s.slot_floats * 4);
+    s.long_floats = 256 * (int64_t)(p.head_dim + 2);
+    s.bytes = s.long_at + (s.may_long ? 2 * kMaxLongParts * ((int64_t)sizeof(int4) + s.long_floats * 4) : 0);
     return s;
 }
 
 template <typename T, int D>
-cudaError_t launch(const kg_pool &p, AttendArgs a, cudaStream_t s) {
+cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *workspace, cudaStream_t s) {
     KvMaps maps;
     std::memset(&maps, 0, sizeof(maps));
     if (!pool_map(&maps.k, p, p.k) || !pool_map(&maps.v, p, p.v)) return cudaErrorInvalidValue;
@@ -441,12 +399,23 @@ cudaError_t launch(const kg_pool &p, AttendArgs a, cudaStream_t s) {
     cudaError_t e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
     if (e != cudaSuccess) return e;
     const int parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
-    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a);
-    if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D>, dim3(parts, std::min(a.rows, 16)), dim3(256), 0, s, a, parts);
-    if (e == cudaSuccess && (int64_t)a.total_q * a.s.group > kShortRows) {
-        const dim3 grid((unsigned)(((int64_t)a.total_q * a.s.group * a.s.n_kv + 3) / 4));
-        e = launch_pdl(attend_rows_kernel<T, D>, grid, dim3(128), 0, s, a, p);
+    if (sp.may_long) {
+        AttendArgs b = a;
+        b.meta = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + sp.long_at);
+        b.part = reinterpret_cast<float *>(b.meta + 2 * kMaxLongParts);
+        b.slot_floats = sp.long_floats;
+        b.rows = 256;
+        const int long_parts = std::min(kMaxLongParts, dev::sm_count());
+        e = attend_long(maps, b, std::is_same<T, __nv_bfloat16>::value, D, long_parts, s);
+        if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D, true>, dim3(long_parts, 32), dim3(256), 0, s, b, long_parts);
+        if (e != cudaSuccess) return e;
     }
+    a.meta = static_cast<int4 *>(workspace);
+    a.part = reinterpret_cast<float *>(a.meta + 2 * kMaxParts);
+    a.slot_floats = sp.slot_floats;
+    a.rows = sp.rows;
+    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a);
+    if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D, false>, dim3(parts, std::min(a.rows, 16)), dim3(256), 0, s, a, parts);
     return e;
 }
 
@@ -517,14 +486,10 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
     a.o_head = out_head_stride;
     a.scale = scale * 1.4426950408889634f;
     a.err = ctx->serve_err;
-    a.meta = static_cast<int4 *>(workspace);
-    a.part = reinterpret_cast<float *>(a.meta + 2 * kMaxParts);
-    a.slot_floats = sp.slot_floats;
-    a.rows = sp.rows;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = pool->dtype == KG_DT_BF16;
-    const cudaError_t e = pool->head_dim == 64 ? (bf ? launch<__nv_bfloat16, 64>(*pool, a, s) : launch<__half, 64>(*pool, a, s))
-                                               : (bf ? launch<__nv_bfloat16, 128>(*pool, a, s) : launch<__half, 128>(*pool, a, s));
+    const cudaError_t e = pool->head_dim == 64 ? (bf ? launch<__nv_bfloat16, 64>(*pool, sp, a, workspace, s) : launch<__half, 64>(*pool, sp, a, workspace, s))
+                                               : (bf ? launch<__nv_bfloat16, 128>(*pool, sp, a, workspace, s) : launch<__half, 128>(*pool, sp, a, workspace, s));
     return e == cudaSuccess ? KG_OK : cuda_fail(ctx, e, "kg_pool_attend_dev");
 }
 

@@ -13,7 +13,7 @@
 namespace kg {
 namespace serve {
 
-constexpr int kMaxParts = 512;  // CTAs of one kernel's line (3 per SM of a B200 at most)
+constexpr int kMaxParts = 512, kMaxLongParts = 160;  // CTAs of the two kernels' lines at most (3 and 1 per SM of a B200)
 
 struct AttendArgs {
     Shape s;
@@ -180,6 +180,9 @@ struct Walk {
     __device__ __forceinline__ int slot() const { return p.unit == 0 ? 1 : 0; }
     __device__ __forceinline__ bool ends() const { return p.unit + n == p.units; }
 };
+
+// The long requests' kernel (kg_pool_long.cu), `parts` CTAs.
+cudaError_t attend_long(const KvMaps &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s);
 
 }  // namespace serve
 }  // namespace kg

@@ -1,0 +1,413 @@
+// kg_pool_long.cu — the long requests of kg_pool_attend_dev (more than 64 rows
+// per K/V head: prompt chunks) on tcgen05.
+//
+// An item is 2 x TQ tokens of one K/V head, TQ = floor(128 / group): two tiles of
+// up to 128 rows (token, query head of the group), one row per tensor-memory lane.
+// Per unit of 128 positions and tile t:
+//   S_t = Q_t K^T      (M 128, N 128, both operands in shared memory)
+//   P_t = 2^(S_t - m)  (a thread owns a row: its maximum and sum need no exchange)
+//   O_t += P_t V       (M 128, N head_dim, P_t from tensor memory over S_t)
+// Warps: 0 loads (TMA, one box per page and 64 elements), 1 and 2 issue the MMAs of
+// tile 0 and tile 1 (one issuing thread cannot keep the tensor pipe busy at these
+// tile sizes), 3..6 and 7..10 are the rows of tile 0 and tile 1. While one tile's
+// rows are exponentiated the other tile's products run.
+// A row's O is rescaled only when its maximum has grown by more than 2^8 since the
+// last time: P then reaches at most 2^8, which 16 bits hold as exactly as 1.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+#include <type_traits>
+
+#include "kg_dev.cuh"
+#include "kg_pdl.cuh"
+#include "kg_pool_attn.cuh"
+#include "kg_tc.cuh"
+
+namespace kg {
+namespace serve {
+namespace {
+
+using namespace as;
+
+constexpr int LONG_THREADS = 352, LONG_LEAST = 2;
+constexpr float RESCALE = 8.0f;
+
+template <int D>
+struct LongCfg {
+    static constexpr int HALF = 128 * 128;           // 128 rows x 64 elements
+    static constexpr int OP = HALF * (D / 64);       // a Q tile, or K or V of a unit
+    static constexpr int SLOTS = D == 64 ? 6 : 4;    // K and V in turn
+    static constexpr int BARS = 2 * SLOTS + 2 + 6;
+    static constexpr int SMEM = 1024 + 2 * OP + SLOTS * OP + BARS * 8 + 16;
+};
+
+// all 128 columns of this thread's lane
+__device__ __forceinline__ void ld128(uint32_t taddr, float (&v)[128]) {
+    uint32_t r[128];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 columns, the wait inside
+__device__ __forceinline__ void ld32w(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+struct LongMaps {
+    CUtensorMap q, k, v;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __grid_constant__ LongMaps maps, const AttendArgs a) {
+    using C = LongCfg<D>;
+    extern __shared__ __align__(1024) uint8_t raw[];
+    uint8_t *sm = raw + ((1024u - (sa(raw) & 1023u)) & 1023u);
+    uint8_t *sq = sm, *ring = sm + 2 * C::OP;
+    uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::SLOTS * C::OP), *empty = full + C::SLOTS;
+    uint64_t *qfull = empty + C::SLOTS, *qempty = qfull + 1;
+    uint64_t *sfull = qempty + 1, *pready = sfull + 2, *pvdone = pready + 2;  // [2] each, by tile
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(pvdone + 2);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tslot + 1);
+    __shared__ long long part_sm[LONG_THREADS / 32 + 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+    const int group = a.s.group, tq = a.s.tile / 2;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 2);
+        }
+        mbar_init(qfull, 1);
+        mbar_init(qempty, 2);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sfull[t], 1);
+            mbar_init(&pready[t], 4);
+            mbar_init(&pvdone[t], 1);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    pdl_wait();
+    int req;
+    long long off, units;
+    find_part<LONG_THREADS, true>(a, c, gridDim.x, LONG_LEAST, part_sm, req, off, units);
+    if (threadIdx.x < 2) a.meta[2 * c + threadIdx.x].x = 0;
+    __syncthreads();
+    if (units == 0) return;
+    if (warp == 0) tc::alloc(tslot, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tb = *tslot;
+    Walk<true> w;
+    w.start(a, req, off, units);
+    // units of tile t's rows within the item's run [unit, unit + n): the first n_of(t)
+    auto n_of = [&](int t) {
+        const int first = (w.p.tile * 2 + t) * tq;
+        if (first >= w.q) return 0;
+        const int lim = row_limit(a.s, w.q, w.kv, min(first + tq, w.q) - 1);
+        const int u = lim > 0 ? (lim - 1) / kLongUnit + 1 : 0;
+        return max(0, min(w.n, u - w.p.unit));
+    };
+
+    if (warp == 0) {  // loads
+        const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows, boxes = pages * (D / 64);
+        const int piece = lane % pages, half = lane / pages;
+        const int dst = half * C::HALF + piece * rows * 128;
+        int it = 0, item = 0;
+        bool ok = true;
+        do {
+            if (lane == 0) {
+                ok = mbar_wait(qempty, (item & 1) ^ 1, abort_flag, a.err);
+                if (ok) {
+                    const int first = w.p.tile * 2 * tq, tiles = first + tq < w.q ? 2 : 1;
+                    mbar_expect_tx(qfull, tiles * (D / 64) * tq * group * 128);
+                    for (int t = 0; t < tiles; ++t)
+                        for (int h = 0; h < D / 64; ++h)
+                            tma_load_4d(sq + t * C::OP + h * C::HALF, &maps.q, h * 64, 0, w.p.head, w.q0 + first + t * tq, qfull);
+                }
+            }
+            ok = __shfl_sync(~0u, ok, 0);
+            for (int u = 0; ok && u < w.n; ++u) {
+                const int pos = (w.p.unit + u) * kLongUnit + piece * rows;
+                int page = a.n_pages;  // outside the pool: the box becomes zeros
+                if (lane < boxes && pos < w.kv) {
+                    const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
+                    if (e >= 0 && e < a.n_pages) page = e;
+                    else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+                }
+                for (int kv = 0; ok && kv < 2; ++kv, ++it) {
+                    const int s = it % C::SLOTS;
+                    if (lane == 0) {
+                        ok = mbar_wait(&empty[s], ((it / C::SLOTS) & 1) ^ 1, abort_flag, a.err);
+                        if (ok) mbar_expect_tx(&full[s], C::OP);
+                    }
+                    ok = __shfl_sync(~0u, ok, 0);
+                    if (ok && lane < boxes)
+                        tma_load_4d(ring + s * C::OP + dst, kv ? &maps.v : &maps.k, half * 64, w.p.head, pos % a.page_size, page, &full[s]);
+                }
+            }
+            ++item;
+        } while (ok && w.next(a));
+        if (!ok) drain_loads(full, C::SLOTS, it);
+    } else if (warp <= 2) {  // products of tile t
+        if (lane == 0) {
+            const int t = warp - 1;
+            constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
+            constexpr uint32_t IDS = tc::idesc_f16(FMT, 128, 128), IDO = tc::idesc_f16(FMT, 128, D, 0, 1);
+            const uint32_t S = tb + t * 128, O = tb + 256 + t * 128;
+            int it = 0, item = 0, cnt = 0;
+            bool ok = true;
+            do {
+                ok = mbar_wait(qfull, item & 1, abort_flag, a.err);
+                tc::fence_after();
+                const int n = n_of(t);
+                const uint64_t dq = tc::sdesc_k(sq + t * C::OP);
+                for (int u = 0; ok && u < w.n; ++u) {
+                    int s = it++ % C::SLOTS;
+                    if (!(ok = mbar_wait(&full[s], ((it - 1) / C::SLOTS) & 1, abort_flag, a.err))) break;
+                    if (u < n) {
+                        tc::fence_after();
+                        const uint64_t dk = tc::sdesc_k(ring + s * C::OP);
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
+                            tc::mma_ss(S, dq + o, dk + o, IDS, k != 0);
+                        }
+                        tc::commit(&sfull[t]);
+                        tc::commit(&empty[s]);
+                    } else {
+                        mbar_arrive(&empty[s]);
+                    }
+                    s = it++ % C::SLOTS;
+                    if (!(ok = mbar_wait(&full[s], ((it - 1) / C::SLOTS) & 1, abort_flag, a.err))) break;
+                    if (u < n) {
+                        if (!(ok = mbar_wait(&pready[t], cnt & 1, abort_flag, a.err))) break;
+                        ++cnt;
+                        tc::fence_after();
+                        const uint64_t dv = tc::sdesc_sw128(sa(ring + s * C::OP), C::HALF, 1024);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) tc::mma_ts(O, S + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, (u | k) != 0);
+                        tc::commit(&pvdone[t]);
+                        tc::commit(&empty[s]);
+                    } else {
+                        mbar_arrive(&empty[s]);
+                    }
+                }
+                if (n > 0) tc::commit(qempty);
+                else mbar_arrive(qempty);
+                ++item;
+            } while (ok && w.next(a));
+        }
+    } else {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
+        const int t = warp >= 7, q4 = warp & 3, i = q4 * 32 + lane;
+        const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+        const uint32_t S = tb + t * 128 + lanes, O = tb + 256 + t * 128 + lanes;
+        int cnt = 0;
+        int v_it = 1;  // ring step of the unit's V
+        bool ok = true;
+        do {
+            const int tok = (w.p.tile * 2 + t) * tq + i / group;
+            const bool valid = i < tq * group && tok < w.q;
+            const int lim = valid ? row_limit(a.s, w.q, w.kv, tok) : 0;
+            const int n = n_of(t);
+            float m = -INFINITY, l = 0.0f;
+            for (int u = 0; ok && u < n; ++u, ++cnt) {
+                ok = mbar_wait(&sfull[t], cnt & 1, abort_flag, a.err);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                tc::fence_after();
+                const int p0 = (w.p.unit + u) * kLongUnit;
+                float x[128];
+                ld128(S, x);
+                const int left = lim - p0;  // positions of this unit that the row attends
+                const bool cut = __any_sync(~0u, left < kLongUnit);
+                if (cut) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j) x[j] = j < left ? x[j] : -INFINITY;
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                top = top == -INFINITY ? top : top * a.scale;
+                const bool grow = u == 0 || top > m + RESCALE;
+                if (u == 0) {
+                    m = top;
+                } else if (__any_sync(~0u, grow)) {
+                    const float f = grow ? exp2_approx(m - top) : 1.0f;
+                    if (grow) m = top;
+                    l *= f;
+                    ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    tc::fence_after();
+                    for (int d = 0; d < D; d += 32) {
+                        float o[32];
+                        ld32w(O + d, o);
+                        uint32_t r[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
+                        tc::st32(O + d, r);
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int e = h * 64 + 2 * j;
+                        float p0v = exp2_approx(fmaf(x[e], a.scale, -base)), p1v = exp2_approx(fmaf(x[e + 1], a.scale, -base));
+                        if (cut) {
+                            p0v = e < left ? p0v : 0.0f;
+                            p1v = e + 1 < left ? p1v : 0.0f;
+                        }
+                        sum[(2 * j) & 3] += p0v;
+                        sum[(2 * j + 1) & 3] += p1v;
+                        pk[j] = Cvt<T>::pack(p0v, p1v);
+                    }
+                    tc::st32(S + h * 32, pk);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (p0 + kLongUnit > w.kv) {  // V rows behind the last position: whatever the page holds must not reach the sums
+                    const int it = v_it + 2 * u, s = it % C::SLOTS;
+                    ok = __all_sync(~0u, mbar_wait(&full[s], (it / C::SLOTS) & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    const int r0 = max(w.kv - p0, 0);
+                    for (int e = i; e < (kLongUnit - r0) * (D / 8); e += 128) {
+                        const int r = r0 + e / (D / 8), ch = e % (D / 8);
+                        *reinterpret_cast<uint4 *>(ring + s * C::OP + (ch >> 3) * C::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                }
+                tc::st_wait();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pready[t]);
+            }
+            // the item's rows
+            if (ok && n > 0) ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
+            if (!ok) break;
+            tc::fence_after();
+            const bool whole = w.whole();
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const int slot = 2 * c + w.slot(), row = t * 128 + i;
+            float *part = a.part + slot * a.slot_floats;
+            T *dst = static_cast<T *>(a.out) + (int64_t)(w.q0 + tok) * a.o_row + (w.p.head * group + i % group) * a.o_head;
+            for (int d = 0; d < D; d += 32) {
+                float o[32];
+                if (n > 0) {
+                    ld32w(O + d, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                }
+                if (valid && whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4 *>(dst + d + e) =
+                            make_uint4(Cvt<T>::pack(o[e] * inv, o[e + 1] * inv), Cvt<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
+                                       Cvt<T>::pack(o[e + 4] * inv, o[e + 5] * inv), Cvt<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+                } else if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(part + (int64_t)row * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+                __syncwarp();
+            }
+            tc::fence_before();
+            if (!whole) {
+                if (valid) reinterpret_cast<float2 *>(part + (int64_t)a.rows * D)[row] = make_float2(m, l);
+                if (i == 0 && t == 0) a.meta[slot] = make_int4(w.ends() ? 3 : 1, w.r, w.p.head, w.p.tile);
+            }
+            v_it += 2 * w.n;
+        } while (w.next(a));
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tb, 512);
+    }
+}
+
+// q as [rows][K/V heads][group][head_dim]: a box is TQ tokens' rows of one K/V
+// head, 64 elements wide, in the order of the tile's rows.
+bool q_map(CUtensorMap *m, const AttendArgs &a, int d) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const int tq = a.s.tile / 2;
+    const int64_t head = a.s.group * a.s.n_kv > 1 ? a.q_head : d, row = a.total_q > 1 ? a.q_row : d;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)a.s.group, (cuuint64_t)a.s.n_kv, (cuuint64_t)a.total_q};
+    const cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)(head * a.s.group) * 2, (cuuint64_t)row * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)a.s.group, 1, (cuuint32_t)tq}, es[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(a.q), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+cudaError_t launch(const KvMaps &kv, const AttendArgs &a, int parts, cudaStream_t s) {
+    LongMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    maps.k = kv.k;
+    maps.v = kv.v;
+    if (!q_map(&maps.q, a, D)) return cudaErrorInvalidValue;
+    using C = LongCfg<D>;
+    cudaError_t e = dev::smem(attend_long_kernel<T, D>, C::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(attend_long_kernel<T, D>, dim3(parts), dim3(LONG_THREADS), C::SMEM, s, maps, a);
+}
+
+}  // namespace
+
+cudaError_t attend_long(const KvMaps &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s) {
+    if (head_dim == 64) return bf16 ? launch<__nv_bfloat16, 64>(kv, a, parts, s) : launch<__half, 64>(kv, a, parts, s);
+    return bf16 ? launch<__nv_bfloat16, 128>(kv, a, parts, s) : launch<__half, 128>(kv, a, parts, s);
+}
+
+}  // namespace serve
+}  // namespace kg
