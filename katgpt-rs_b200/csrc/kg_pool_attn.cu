@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cstring>
 #include <type_traits>
 
@@ -484,7 +485,7 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
     a.q_head = q_head_stride;
     a.o_row = out_row_stride;
     a.o_head = out_head_stride;
-    a.scale = scale * 1.4426950408889634f;
+    a.scale = std::max(scale * 1.4426950408889634f, FLT_MIN);  // (a masked score, -inf, times 0 would be NaN)
     a.err = ctx->serve_err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = pool->dtype == KG_DT_BF16;

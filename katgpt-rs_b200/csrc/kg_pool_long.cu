@@ -9,7 +9,7 @@
 //   O_t += P_t V       (M 128, N head_dim, P_t from tensor memory over S_t)
 // Warps: 0 loads (TMA, one box per page and 64 elements), 1 and 2 issue the MMAs of
 // tile 0 and tile 1 (one issuing thread cannot keep the tensor pipe busy at these
-// tile sizes), 3..6 and 7..10 are the rows of tile 0 and tile 1. While one tile's
+// tile sizes), 4..7 and 8..11 are the rows of tile 0 and tile 1. While one tile's
 // rows are exponentiated the other tile's products run.
 // A row's O is rescaled only when its maximum has grown by more than 2^8 since the
 // last time: P then reaches at most 2^8, which 16 bits hold as exactly as 1.
@@ -32,7 +32,10 @@ namespace {
 
 using namespace as;
 
-constexpr int LONG_THREADS = 352, LONG_LEAST = 2;
+constexpr int LONG_THREADS = 384, LONG_LEAST = 2;
+// registers: 384 threads start with 168 each; four warps keep 80, eight take 208 (128 * 80 + 256 * 208 <= 384 * 168)
+constexpr int REGS_FEW = 80, REGS_MANY = 208;
+static_assert(128 * REGS_FEW + 256 * REGS_MANY <= LONG_THREADS * 168, "register split");
 constexpr float RESCALE = 8.0f;
 
 template <int D>
@@ -40,7 +43,7 @@ struct LongCfg {
     static constexpr int HALF = 128 * 128;           // 128 rows x 64 elements
     static constexpr int OP = HALF * (D / 64);       // a Q tile, or K or V of a unit
     static constexpr int SLOTS = D == 64 ? 6 : 4;    // K and V in turn
-    static constexpr int BARS = 2 * SLOTS + 2 + 6;
+    static constexpr int BARS = 2 * SLOTS + 2 + 8;
     static constexpr int SMEM = 1024 + 2 * OP + SLOTS * OP + BARS * 8 + 16;
 };
 
@@ -78,21 +81,38 @@ __device__ __forceinline__ void ld128(uint32_t taddr, float (&v)[128]) {
 #pragma unroll
     for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
-// 32 columns, the wait inside
-__device__ __forceinline__ void ld32w(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
+// 16 columns, the wait inside
+__device__ __forceinline__ void ld16w(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
         "tcgen05.wait::ld.sync.aligned;\n"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// two f32 at a time
+__device__ __forceinline__ unsigned long long two(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void halves(unsigned long long v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 struct LongMaps {
@@ -107,8 +127,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     uint8_t *sq = sm, *ring = sm + 2 * C::OP;
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::SLOTS * C::OP), *empty = full + C::SLOTS;
     uint64_t *qfull = empty + C::SLOTS, *qempty = qfull + 1;
-    uint64_t *sfull = qempty + 1, *pready = sfull + 2, *pvdone = pready + 2;  // [2] each, by tile
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(pvdone + 2);
+    uint64_t *sfull = qempty + 1, *pvdone = sfull + 2, *pready = pvdone + 2;  // [2] by tile, pready [tile][half]
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(pready + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tslot + 1);
     __shared__ long long part_sm[LONG_THREADS / 32 + 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
@@ -122,7 +142,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         mbar_init(qempty, 2);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sfull[t], 1);
-            mbar_init(&pready[t], 4);
+            mbar_init(&pready[2 * t], 4);
+            mbar_init(&pready[2 * t + 1], 4);
             mbar_init(&pvdone[t], 1);
         }
         *abort_flag = 0;
@@ -151,6 +172,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         return max(0, min(w.n, u - w.p.unit));
     };
 
+    if (warp < 4) regs_down<REGS_FEW>();
+    else regs_up<REGS_MANY>();
     if (warp == 0) {  // loads
         const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows, boxes = pages * (D / 64);
         const int piece = lane % pages, half = lane / pages;
@@ -223,12 +246,17 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     s = it++ % C::SLOTS;
                     if (!(ok = mbar_wait(&full[s], ((it - 1) / C::SLOTS) & 1, abort_flag, a.err))) break;
                     if (u < n) {
-                        if (!(ok = mbar_wait(&pready[t], cnt & 1, abort_flag, a.err))) break;
-                        ++cnt;
-                        tc::fence_after();
                         const uint64_t dv = tc::sdesc_sw128(sa(ring + s * C::OP), C::HALF, 1024);
+                        // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) tc::mma_ts(O, S + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, (u | k) != 0);
+                        for (int h = 0; h < 2; ++h) {
+                            if (!(ok = mbar_wait(&pready[2 * t + h], cnt & 1, abort_flag, a.err))) break;
+                            tc::fence_after();
+#pragma unroll
+                            for (int k = h * 4; k < h * 4 + 4; ++k) tc::mma_ts(O, S + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, (u | k) != 0);
+                        }
+                        if (!ok) break;
+                        ++cnt;
                         tc::commit(&pvdone[t]);
                         tc::commit(&empty[s]);
                     } else {
@@ -240,8 +268,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 ++item;
             } while (ok && w.next(a));
         }
-    } else {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
-        const int t = warp >= 7, q4 = warp & 3, i = q4 * 32 + lane;
+    } else if (warp >= 4) {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
+        const int t = warp >= 8, q4 = warp & 3, i = q4 * 32 + lane;
         const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
         const uint32_t S = tb + t * 128 + lanes, O = tb + 256 + t * 128 + lanes;
         int cnt = 0;
@@ -269,7 +297,11 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 }
                 float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], x[j]);
+                for (int j = 4; j < 124; j += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], x[j + 2 * k]), x[j + 2 * k + 1]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[124 + k]);
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 top = top == -INFINITY ? top : top * a.scale;
                 const bool grow = u == 0 || top > m + RESCALE;
@@ -282,35 +314,15 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
                     if (!ok) break;
                     tc::fence_after();
-                    for (int d = 0; d < D; d += 32) {
-                        float o[32];
-                        ld32w(O + d, o);
-                        uint32_t r[32];
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 16) {
+                        uint32_t r[16];
+                        ld16w(O + d, r);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
-                        tc::st32(O + d, r);
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                        tc::st16(O + d, r);
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int e = h * 64 + 2 * j;
-                        float p0v = exp2_approx(fmaf(x[e], a.scale, -base)), p1v = exp2_approx(fmaf(x[e + 1], a.scale, -base));
-                        if (cut) {
-                            p0v = e < left ? p0v : 0.0f;
-                            p1v = e + 1 < left ? p1v : 0.0f;
-                        }
-                        sum[(2 * j) & 3] += p0v;
-                        sum[(2 * j + 1) & 3] += p1v;
-                        pk[j] = Cvt<T>::pack(p0v, p1v);
-                    }
-                    tc::st32(S + h * 32, pk);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (p0 + kLongUnit > w.kv) {  // V rows behind the last position: whatever the page holds must not reach the sums
                     const int it = v_it + 2 * u, s = it % C::SLOTS;
                     ok = __all_sync(~0u, mbar_wait(&full[s], (it / C::SLOTS) & 1, abort_flag, a.err));
@@ -323,10 +335,34 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     tc::fence_proxy_async();
                     __syncwarp();
                 }
-                tc::st_wait();
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&pready[t]);
+                const float base = m == -INFINITY ? 0.0f : m;
+                const unsigned long long scale2 = two(a.scale, a.scale), base2 = two(-base, -base);
+                unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int e = h * 64 + g * 32 + 2 * j;
+                            float pa, pb;
+                            halves(fma2(two(x[e], x[e + 1]), scale2, base2), pa, pb);
+                            pa = exp2_approx(pa);
+                            pb = exp2_approx(pb);
+                            sum[j & 1] = add2(sum[j & 1], two(pa, pb));
+                            pk[j] = Cvt<T>::pack(pa, pb);
+                        }
+                        tc::st16(S + h * 32 + g * 16, pk);
+                    }
+                    tc::st_wait();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pready[2 * t + h]);
+                }
+                float s0, s1;
+                halves(add2(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
             }
             // the item's rows
             if (ok && n > 0) ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
@@ -337,23 +373,22 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             const int slot = 2 * c + w.slot(), row = t * 128 + i;
             float *part = a.part + slot * a.slot_floats;
             T *dst = static_cast<T *>(a.out) + (int64_t)(w.q0 + tok) * a.o_row + (w.p.head * group + i % group) * a.o_head;
-            for (int d = 0; d < D; d += 32) {
-                float o[32];
-                if (n > 0) {
-                    ld32w(O + d, o);
-                } else {
+#pragma unroll 2
+            for (int d = 0; d < D; d += 16) {
+                uint32_t r[16] = {};
+                float o[16];
+                if (n > 0) ld16w(O + d, r);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-                }
+                for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(r[e]);
                 if (valid && whole) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
+                    for (int e = 0; e < 16; e += 8)
                         *reinterpret_cast<uint4 *>(dst + d + e) =
                             make_uint4(Cvt<T>::pack(o[e] * inv, o[e + 1] * inv), Cvt<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
                                        Cvt<T>::pack(o[e + 4] * inv, o[e + 5] * inv), Cvt<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
                 } else if (valid) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
+                    for (int e = 0; e < 16; e += 4)
                         *reinterpret_cast<float4 *>(part + (int64_t)row * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
                 __syncwarp();
