@@ -7,10 +7,12 @@
 //   S_t = Q_t K^T      (M 128, N 128, both operands in shared memory)
 //   P_t = 2^(S_t - m)  (a thread owns a row: its maximum and sum need no exchange)
 //   O_t += P_t V       (M 128, N head_dim, P_t from tensor memory over S_t)
-// Warps: 0 loads (TMA, one box per page and 64 elements), 1 and 2 issue the MMAs of
-// tile 0 and tile 1 (one issuing thread cannot keep the tensor pipe busy at these
-// tile sizes), 4..7 and 8..11 are the rows of tile 0 and tile 1. While one tile's
-// rows are exponentiated the other tile's products run.
+// Warps: 0 loads (TMA, one box per page and 64 elements), 1 issues the products, 2..5
+// and 6..9 are the rows of tile 0 and tile 1. The products go P_0 V, Q_0 K^T, P_1 V,
+// Q_1 K^T in turn from one thread, so that the tiles stay half a step apart: one tile's
+// rows are exponentiated while the other tile's products run. (Two issuing threads let
+// the tiles fall into step, both waiting for the tensor pipe and then both for the
+// exponentials: 4640 cycles a pair of units at 1.70 GHz.)
 // A row's O is rescaled only when its maximum has grown by more than 2^8 since the
 // last time: P then reaches at most 2^8, which 16 bits hold as exactly as 1.
 #include <cuda_bf16.h>
@@ -32,10 +34,7 @@ namespace {
 
 using namespace as;
 
-constexpr int LONG_THREADS = 384, LONG_LEAST = 2;
-// registers: 384 threads start with 168 each; four warps keep 80, eight take 208 (128 * 80 + 256 * 208 <= 384 * 168)
-constexpr int REGS_FEW = 80, REGS_MANY = 208;
-static_assert(128 * REGS_FEW + 256 * REGS_MANY <= LONG_THREADS * 168, "register split");
+constexpr int LONG_THREADS = 320, LONG_LEAST = 2;
 constexpr float RESCALE = 8.0f;
 
 template <int D>
@@ -92,11 +91,6 @@ __device__ __forceinline__ void ld16w(uint32_t taddr, uint32_t (&r)[16]) {
         : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
 // two f32 at a time
 __device__ __forceinline__ unsigned long long two(float x, float y) {
     unsigned long long r;
@@ -136,10 +130,10 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 2);
+            mbar_init(&empty[i], 1);
         }
         mbar_init(qfull, 1);
-        mbar_init(qempty, 2);
+        mbar_init(qempty, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sfull[t], 1);
             mbar_init(&pready[2 * t], 4);
@@ -172,8 +166,6 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         return max(0, min(w.n, u - w.p.unit));
     };
 
-    if (warp < 4) regs_down<REGS_FEW>();
-    else regs_up<REGS_MANY>();
     if (warp == 0) {  // loads
         const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows, boxes = pages * (D / 64);
         const int piece = lane % pages, half = lane / pages;
@@ -214,62 +206,69 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             ++item;
         } while (ok && w.next(a));
         if (!ok) drain_loads(full, C::SLOTS, it);
-    } else if (warp <= 2) {  // products of tile t
+    } else if (warp == 1) {  // products, tile 0 and tile 1 in turn
         if (lane == 0) {
-            const int t = warp - 1;
             constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
             constexpr uint32_t IDS = tc::idesc_f16(FMT, 128, 128), IDO = tc::idesc_f16(FMT, 128, D, 0, 1);
-            const uint32_t S = tb + t * 128, O = tb + 256 + t * 128;
-            int it = 0, item = 0, cnt = 0;
+            int it = 0, item = 0, cnt[2] = {0, 0};
             bool ok = true;
-            do {
-                ok = mbar_wait(qfull, item & 1, abort_flag, a.err);
-                tc::fence_after();
-                const int n = n_of(t);
-                const uint64_t dq = tc::sdesc_k(sq + t * C::OP);
-                for (int u = 0; ok && u < w.n; ++u) {
-                    int s = it++ % C::SLOTS;
-                    if (!(ok = mbar_wait(&full[s], ((it - 1) / C::SLOTS) & 1, abort_flag, a.err))) break;
-                    if (u < n) {
-                        tc::fence_after();
-                        const uint64_t dk = tc::sdesc_k(ring + s * C::OP);
+            auto wait_slot = [&](int step) { return mbar_wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1, abort_flag, a.err); };
+            auto scores = [&](int t, int step) {
+                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_k(ring + step % C::SLOTS * C::OP);
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
-                            tc::mma_ss(S, dq + o, dk + o, IDS, k != 0);
-                        }
-                        tc::commit(&sfull[t]);
-                        tc::commit(&empty[s]);
-                    } else {
-                        mbar_arrive(&empty[s]);
-                    }
-                    s = it++ % C::SLOTS;
-                    if (!(ok = mbar_wait(&full[s], ((it - 1) / C::SLOTS) & 1, abort_flag, a.err))) break;
-                    if (u < n) {
-                        const uint64_t dv = tc::sdesc_sw128(sa(ring + s * C::OP), C::HALF, 1024);
-                        // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (!(ok = mbar_wait(&pready[2 * t + h], cnt & 1, abort_flag, a.err))) break;
-                            tc::fence_after();
-#pragma unroll
-                            for (int k = h * 4; k < h * 4 + 4; ++k) tc::mma_ts(O, S + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, (u | k) != 0);
-                        }
-                        if (!ok) break;
-                        ++cnt;
-                        tc::commit(&pvdone[t]);
-                        tc::commit(&empty[s]);
-                    } else {
-                        mbar_arrive(&empty[s]);
-                    }
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
+                    tc::mma_ss(tb + t * 128, dq + o, dk + o, IDS, k != 0);
                 }
-                if (n > 0) tc::commit(qempty);
+                tc::commit(&sfull[t]);
+            };
+            auto values = [&](int t, int step, bool first) {
+                const uint64_t dv = tc::sdesc_sw128(sa(ring + step % C::SLOTS * C::OP), C::HALF, 1024);
+                // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!mbar_wait(&pready[2 * t + h], cnt[t] & 1, abort_flag, a.err)) return false;
+                    tc::fence_after();
+#pragma unroll
+                    for (int k = h * 4; k < h * 4 + 4; ++k)
+                        tc::mma_ts(tb + 256 + t * 128, tb + t * 128 + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, !(first && k == 0));
+                }
+                ++cnt[t];
+                tc::commit(&pvdone[t]);
+                return true;
+            };
+            // a slot is free once the products that read it are done
+            auto release = [&](int step, bool used) {
+                if (used) tc::commit(&empty[step % C::SLOTS]);
+                else mbar_arrive(&empty[step % C::SLOTS]);
+            };
+            do {
+                const int n0 = n_of(0), n1 = n_of(1);
+                if (!(ok = mbar_wait(qfull, item & 1, abort_flag, a.err) && wait_slot(it))) break;
+                tc::fence_after();
+                if (n0 > 0) scores(0, it);
+                if (n1 > 0) scores(1, it);
+                release(it, n0 > 0 || n1 > 0);
+                for (int u = 0; ok && u < w.n; ++u, it += 2) {
+                    const bool more = u + 1 < w.n;
+                    if (!(ok = wait_slot(it + 1))) break;
+                    tc::fence_after();
+                    if (u < n0 && !(ok = values(0, it + 1, u == 0))) break;
+                    if (more && !(ok = wait_slot(it + 2))) break;
+                    tc::fence_after();
+                    if (u + 1 < n0) scores(0, it + 2);
+                    if (u < n1 && !(ok = values(1, it + 1, u == 0))) break;
+                    release(it + 1, u < n0 || u < n1);
+                    if (u + 1 < n1) scores(1, it + 2);
+                    if (more) release(it + 2, u + 1 < n0 || u + 1 < n1);
+                }
+                if (n0 > 0 || n1 > 0) tc::commit(qempty);
                 else mbar_arrive(qempty);
                 ++item;
             } while (ok && w.next(a));
         }
-    } else if (warp >= 4) {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
-        const int t = warp >= 8, q4 = warp & 3, i = q4 * 32 + lane;
+    } else {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
+        const int t = warp >= 6, q4 = warp & 3, i = q4 * 32 + lane;
         const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
         const uint32_t S = tb + t * 128 + lanes, O = tb + 256 + t * 128 + lanes;
         int cnt = 0;
