@@ -46,18 +46,14 @@ struct LongCfg {
     static constexpr int SMEM = 1024 + 2 * OP + SLOTS * OP + BARS * 8 + 16;
 };
 
-// all 128 columns of this thread's lane
-__device__ __forceinline__ void ld128(uint32_t taddr, float (&v)[128]) {
-    uint32_t r[128];
+// 64 columns of this thread's lane, the wait inside
+__device__ __forceinline__ void ld64w(uint32_t taddr, float (&v)[64]) {
+    uint32_t r[64];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
         "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
         "tcgen05.wait::ld.sync.aligned;\n"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -66,19 +62,11 @@ __device__ __forceinline__ void ld128(uint32_t taddr, float (&v)[128]) {
           "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
           "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
           "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
         : "r"(taddr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 // 16 columns, the wait inside
 __device__ __forceinline__ void ld16w(uint32_t taddr, uint32_t (&r)[16]) {
@@ -90,6 +78,14 @@ __device__ __forceinline__ void ld16w(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr)
         : "memory");
 }
+
+// one lane of a converged warp, always the same one (its products stay in order)
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred P;\n elect.sync _|P, 0xffffffff;\n selp.u32 %0, 1, 0, P;\n}\n" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(~0u, x, 0); }
 
 // two f32 at a time
 __device__ __forceinline__ unsigned long long two(float x, float y) {
@@ -125,7 +121,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     uint32_t *tslot = reinterpret_cast<uint32_t *>(pready + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tslot + 1);
     __shared__ long long part_sm[LONG_THREADS / 32 + 2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, c = blockIdx.x;
     const int group = a.s.group, tq = a.s.tile / 2;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::SLOTS; ++i) {
@@ -207,44 +203,56 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         } while (ok && w.next(a));
         if (!ok) drain_loads(full, C::SLOTS, it);
     } else if (warp == 1) {  // products, tile 0 and tile 1 in turn
-        if (lane == 0) {
+        // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers. From inside a
+        // one-lane branch a product took about 110 cycles to issue, against 64 to run.
+        {
             constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
             constexpr uint32_t IDS = tc::idesc_f16(FMT, 128, 128), IDO = tc::idesc_f16(FMT, 128, D, 0, 1);
             int it = 0, item = 0, cnt[2] = {0, 0};
             bool ok = true;
-            auto wait_slot = [&](int step) { return mbar_wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1, abort_flag, a.err); };
+            auto wait = [&](uint64_t *b, int parity) { return __all_sync(~0u, mbar_wait(b, parity, abort_flag, a.err)) != 0; };
+            auto wait_slot = [&](int step) { return wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1); };
             auto scores = [&](int t, int step) {
-                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_k(ring + step % C::SLOTS * C::OP);
+                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_k(ring + uniform(step % C::SLOTS) * C::OP);
+                if (elect()) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
-                    tc::mma_ss(tb + t * 128, dq + o, dk + o, IDS, k != 0);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
+                        tc::mma_ss(tb + t * 128, dq + o, dk + o, IDS, k != 0);
+                    }
+                    tc::commit(&sfull[t]);
                 }
-                tc::commit(&sfull[t]);
+                __syncwarp();
             };
             auto values = [&](int t, int step, bool first) {
-                const uint64_t dv = tc::sdesc_sw128(sa(ring + step % C::SLOTS * C::OP), C::HALF, 1024);
+                const uint64_t dv = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), C::HALF, 1024);
                 // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if (!mbar_wait(&pready[2 * t + h], cnt[t] & 1, abort_flag, a.err)) return false;
+                    if (!wait(&pready[2 * t + h], cnt[t] & 1)) return false;
                     tc::fence_after();
+                    if (elect()) {
 #pragma unroll
-                    for (int k = h * 4; k < h * 4 + 4; ++k)
-                        tc::mma_ts(tb + 256 + t * 128, tb + t * 128 + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, !(first && k == 0));
+                        for (int k = h * 4; k < h * 4 + 4; ++k)
+                            tc::mma_ts(tb + 256 + t * 128, tb + t * 128 + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, !(first && k == 0));
+                        if (h == 1) tc::commit(&pvdone[t]);
+                    }
+                    __syncwarp();
                 }
                 ++cnt[t];
-                tc::commit(&pvdone[t]);
                 return true;
             };
             // a slot is free once the products that read it are done
             auto release = [&](int step, bool used) {
-                if (used) tc::commit(&empty[step % C::SLOTS]);
-                else mbar_arrive(&empty[step % C::SLOTS]);
+                if (elect()) {
+                    if (used) tc::commit(&empty[step % C::SLOTS]);
+                    else mbar_arrive(&empty[step % C::SLOTS]);
+                }
+                __syncwarp();
             };
             do {
                 const int n0 = n_of(0), n1 = n_of(1);
-                if (!(ok = mbar_wait(qfull, item & 1, abort_flag, a.err) && wait_slot(it))) break;
+                if (!(ok = wait(qfull, item & 1) && wait_slot(it))) break;
                 tc::fence_after();
                 if (n0 > 0) scores(0, it);
                 if (n1 > 0) scores(1, it);
@@ -262,8 +270,11 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     if (u + 1 < n1) scores(1, it + 2);
                     if (more) release(it + 2, u + 1 < n0 || u + 1 < n1);
                 }
-                if (n0 > 0 || n1 > 0) tc::commit(qempty);
-                else mbar_arrive(qempty);
+                if (elect()) {
+                    if (n0 > 0 || n1 > 0) tc::commit(qempty);
+                    else mbar_arrive(qempty);
+                }
+                __syncwarp();
                 ++item;
             } while (ok && w.next(a));
         }
@@ -286,22 +297,31 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 if (!ok) break;
                 tc::fence_after();
                 const int p0 = (w.p.unit + u) * kLongUnit;
-                float x[128];
-                ld128(S, x);
                 const int left = lim - p0;  // positions of this unit that the row attends
                 const bool cut = __any_sync(~0u, left < kLongUnit);
-                if (cut) {
+                // 64 scores in registers at a time: the second half is read for the maximum, and again after the first is done
+                float x[64];
+                auto half = [&](int h) {
+                    ld64w(S + h * 64, x);
+                    if (cut) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j) x[j] = j < left ? x[j] : -INFINITY;
-                }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
+                        for (int j = 0; j < 64; ++j) x[j] = h * 64 + j < left ? x[j] : -INFINITY;
+                    }
+                };
+                auto top_of = [&]() {
+                    float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int j = 4; j < 124; j += 8)
+                    for (int j = 4; j < 60; j += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], x[j + 2 * k]), x[j + 2 * k + 1]);
+                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], x[j + 2 * k]), x[j + 2 * k + 1]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[124 + k]);
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[60 + k]);
+                    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                };
+                half(1);
+                float top = top_of();
+                half(0);
+                top = fmaxf(top, top_of());
                 top = top == -INFINITY ? top : top * a.scale;
                 const bool grow = u == 0 || top > m + RESCALE;
                 if (u == 0) {
@@ -339,12 +359,13 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 unsigned long long sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    if (h == 1) half(1);
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const int e = h * 64 + g * 32 + 2 * j;
+                            const int e = g * 32 + 2 * j;
                             float pa, pb;
                             halves(fma2(two(x[e], x[e + 1]), scale2, base2), pa, pb);
                             pa = exp2_approx(pa);
