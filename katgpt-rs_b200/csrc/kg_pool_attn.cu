@@ -37,8 +37,7 @@ constexpr int SHORT_THREADS = 160, SHORT_LEAST = 2;
 
 template <int D>
 struct ShortCfg {
-    static constexpr int HALF_BYTES = kShortUnit * 128;              // 64 positions x 64 elements
-    static constexpr int OP_BYTES = HALF_BYTES * (D / 64);           // K or V of a stage
+    static constexpr int OP_BYTES = kShortUnit * D * 2;  // K or V of a stage
     static constexpr int STAGES = D == 64 ? 4 : 3;
     static constexpr int SCRATCH = 4 * 16 * 36 * 4;
     static constexpr int SMEM = 1024 + STAGES * 2 * OP_BYTES + SCRATCH + 4 * 16 * 2 * 4 + 2 * STAGES * 8 + 16;
@@ -71,7 +70,7 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ KvMaps maps, const AttendArgs a) {
+__global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ PoolMap maps, const AttendArgs a) {
     using C = ShortCfg<D>;
     extern __shared__ __align__(1024) uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (sa(raw) & 1023u)) & 1023u);
@@ -100,18 +99,18 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     w.start(a, req, off, units);
 
     if (warp == 4) {  // producer: lane i loads box i of a unit
-        const int rows = min(a.page_size, kShortUnit), pages = kShortUnit / rows, boxes = pages * (D / 64) * 2;
-        const int piece = lane % pages, half = lane / pages % (D / 64), which = lane / (pages * (D / 64));
+        const int rows = min(a.page_size, kShortUnit), pages = kShortUnit / rows, boxes = pages * 2;
+        const int piece = lane % pages, which = lane / pages;
         const CUtensorMap *tm = which ? &maps.v : &maps.k;
-        const int dst = which * C::OP_BYTES + half * C::HALF_BYTES + piece * rows * 128;
+        const int dst = which * C::OP_BYTES + piece * rows * D * 2;
         int it = 0;
         do {
             for (int u = 0; u < w.n; ++u, ++it) {
                 const int s = it % C::STAGES, pos = (w.p.unit + u) * kShortUnit + piece * rows;
-                int page = a.n_pages;  // outside the pool: the box becomes zeros
+                int place = maps.outside;
                 if (lane < boxes && pos < w.kv) {
                     const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
-                    if (e >= 0 && e < a.n_pages) page = e;
+                    if (e >= 0 && e < a.n_pages) place = e * maps.page_step + w.p.head * maps.head_step;
                     else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
                 }
                 int ok = 1;
@@ -124,7 +123,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                     return;
                 }
                 if (lane < boxes)
-                    tma_load_4d(sm + s * 2 * C::OP_BYTES + dst, tm, half * 64, w.p.head, pos % a.page_size, page, &full[s]);
+                    tma_load_5d(sm + s * 2 * C::OP_BYTES + dst, tm, pos % a.page_size / 8, place, &full[s]);
             }
         } while (w.next(a));
         return;
@@ -167,8 +166,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                     for (int i = lane; i < 16 * (D / 8); i += 32) {
                         const int r = i / (D / 8), ch = i % (D / 8);
                         if (pos0 + r >= w.kv)
-                            *reinterpret_cast<uint4 *>(st + C::OP_BYTES + (ch >> 3) * C::HALF_BYTES + (p0 + r) * 128 + (ch & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4 *>(st + C::OP_BYTES + kv_offset<D>(p0 + r, ch)) = make_uint4(0, 0, 0, 0);
                     }
                     wrote = true;
                     __syncwarp();
@@ -176,12 +174,12 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                 float sc[2][4] = {};
                 {
                     const int r = p0 + (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
-                    const uint32_t base = sa(st) + r * 128;
+                    const uint32_t base = sa(st) + kv_offset<D>(r, 0);
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const int ch = k * 2 + cb;
                         uint32_t kf[4];
-                        ldsm4(base + (ch >> 3) * C::HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4), kf);
+                        ldsm4(base + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), kf);
                         mma16816<T>(sc[0], qf[k], kf[0], kf[1]);
                         mma16816<T>(sc[1], qf[k], kf[2], kf[3]);
                     }
@@ -218,12 +216,12 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                 }
                 {
                     const int r = p0 + (lane & 7) + (((lane >> 3) & 1) << 3), cb = lane >> 4;
-                    const uint32_t base = sa(st) + C::OP_BYTES + r * 128;
+                    const uint32_t base = sa(st) + C::OP_BYTES + kv_offset<D>(r, 0);
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const int ch = k * 2 + cb;
                         uint32_t vf[4];
-                        ldsm4t(base + (ch >> 3) * C::HALF_BYTES + (((ch & 7) ^ (r & 7)) << 4), vf);
+                        ldsm4t(base + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), vf);
                         mma16816<T>(o[2 * k], pf, vf[0], vf[1]);
                         mma16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
                     }
@@ -358,18 +356,23 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, in
 // ---------------------------------------------------------------------------
 // Host
 
-// The pool as [pages][page rows][heads][head_dim], boxes of one page's rows (64
-// at most), one head and 64 elements (128 bytes, the swizzle's width).
-bool pool_map(CUtensorMap *m, const kg_pool &p, const void *base) {
+// The pool's maps (PoolMap); false when the driver refuses them.
+bool pool_map(PoolMap &m, const kg_pool &p) {
     auto fn = tensor_map_encoder();
     if (!fn) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_kv_head, (cuuint64_t)p.page_size, (cuuint64_t)p.n_pages};
-    auto bytes = [&](int64_t stride, int64_t count) { return (cuuint64_t)(count > 1 ? stride : p.head_dim) * 2; };
-    const cuuint64_t strides[3] = {bytes(p.head_stride, p.n_kv_head), bytes(p.row_stride, p.page_size), bytes(p.page_stride, p.n_pages)};
-    const cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(p.page_size, kShortUnit), 1}, es[4] = {1, 1, 1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const int64_t unit = pool_unit(p), rs = p.row_stride;
+    m.page_step = (int)(p.n_pages > 1 ? p.page_stride / unit : 0);
+    m.head_step = (int)(p.n_kv_head > 1 ? p.head_stride / unit : 0);
+    m.outside = (p.n_pages - 1) * m.page_step + (p.n_kv_head - 1) * m.head_step + 1;
+    const cuuint64_t dims[5] = {64, 8, (cuuint64_t)p.head_dim / 64, (cuuint64_t)p.page_size / 8, (cuuint64_t)m.outside};
+    const cuuint64_t strides[4] = {(cuuint64_t)rs * 2, 128, (cuuint64_t)rs * 16, (cuuint64_t)unit * 2};
+    const cuuint32_t box[5] = {64, 8, (cuuint32_t)p.head_dim / 64, (cuuint32_t)std::min(p.page_size, kShortUnit) / 8, 1};
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < 2; ++i)
+        if (fn(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, i ? p.v : p.k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
 }
 
 // Workspace: [meta][part sums], for the short requests' kernel and then, where
@@ -393,9 +396,9 @@ Space space_of(const kg_pool &p, int n_head, int total_q) {
 
 template <typename T, int D>
 cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *workspace, cudaStream_t s) {
-    KvMaps maps;
+    PoolMap maps;
     std::memset(&maps, 0, sizeof(maps));
-    if (!pool_map(&maps.k, p, p.k) || !pool_map(&maps.v, p, p.v)) return cudaErrorInvalidValue;
+    if (!pool_map(maps, p)) return cudaErrorInvalidValue;
     using C = ShortCfg<D>;
     cudaError_t e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
     if (e != cudaSuccess) return e;

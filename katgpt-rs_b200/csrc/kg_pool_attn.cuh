@@ -31,9 +31,6 @@ struct AttendArgs {
     int rows;
     int4 *meta;  // per slot: {0 unused, 1 used, 3 used and the item's end, request, head, tile}
 };
-struct KvMaps {
-    CUtensorMap k, v;
-};
 
 template <typename T>
 struct Cvt;
@@ -68,7 +65,30 @@ __device__ __forceinline__ void drain_loads(uint64_t *full, int stages, int it) 
     }
 }
 
-// 4-D tiled load: one page's rows of one head, 64 elements wide
+// Shared-memory form of K and V: groups of 8 positions, each [head_dim / 64][8
+// rows][128 bytes] with the 128-byte swizzle. One TMA box brings all of a page's
+// rows of one head (64 at most) in this order: the pool is mapped as
+//   [64 elements][8 rows][head_dim / 64][row groups][page and head]
+// where the last axis counts in steps of `unit` elements, the greatest common
+// divisor of the page and head strides. (A box for every 64 elements of a 16-row
+// page, 2 KB each, kept the loads of a prompt chunk behind its products.)
+struct PoolMap {
+    CUtensorMap k, v;
+    int page_step, head_step, outside;  // in the last axis; `outside` lies behind it: such a box becomes zeros
+};
+template <int D>
+__device__ __forceinline__ uint32_t kv_offset(int row, int chunk) {  // of a 16-byte chunk, before the swizzle
+    return (row >> 3) * (D * 16) + (chunk >> 3) * 1024 + (row & 7) * 128 + (chunk & 7) * 16;
+}
+__device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *tm, int row_group, int place, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], "
+        "[%5];\n" ::"r"(as::sa(dst)),
+        "l"(tm), "r"(0), "r"(row_group), "r"(place), "r"(as::sa(bar))
+        : "memory");
+}
+
+// 4-D tiled load: the rows of q of one K/V head, 64 elements wide
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *tm, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
@@ -182,7 +202,7 @@ struct Walk {
 };
 
 // The long requests' kernel (kg_pool_long.cu), `parts` CTAs.
-cudaError_t attend_long(const KvMaps &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s);
+cudaError_t attend_long(const PoolMap &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s);
 
 }  // namespace serve
 }  // namespace kg

@@ -7,7 +7,7 @@
 //   S_t = Q_t K^T      (M 128, N 128, both operands in shared memory)
 //   P_t = 2^(S_t - m)  (a thread owns a row: its maximum and sum need no exchange)
 //   O_t += P_t V       (M 128, N head_dim, P_t from tensor memory over S_t)
-// Warps: 0 loads (TMA, one box per page and 64 elements), 1 issues the products, 2..5
+// Warps: 0 loads (TMA, a box per page), 1 issues the products, 2..5
 // and 6..9 are the rows of tile 0 and tile 1. The products go P_0 V, Q_0 K^T, P_1 V,
 // Q_1 K^T in turn from one thread, so that the tiles stay half a step apart: one tile's
 // rows are exponentiated while the other tile's products run. (Two issuing threads let
@@ -106,7 +106,8 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
 }
 
 struct LongMaps {
-    CUtensorMap q, k, v;
+    CUtensorMap q;
+    PoolMap kv;
 };
 
 template <typename T, int D>
@@ -163,9 +164,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     };
 
     if (warp == 0) {  // loads
-        const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows, boxes = pages * (D / 64);
-        const int piece = lane % pages, half = lane / pages;
-        const int dst = half * C::HALF + piece * rows * 128;
+        const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows;  // a box each
         int it = 0, item = 0;
         bool ok = true;
         do {
@@ -181,11 +180,11 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             }
             ok = __shfl_sync(~0u, ok, 0);
             for (int u = 0; ok && u < w.n; ++u) {
-                const int pos = (w.p.unit + u) * kLongUnit + piece * rows;
-                int page = a.n_pages;  // outside the pool: the box becomes zeros
-                if (lane < boxes && pos < w.kv) {
+                const int pos = (w.p.unit + u) * kLongUnit + lane * rows;
+                int place = maps.kv.outside;
+                if (lane < pages && pos < w.kv) {
                     const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
-                    if (e >= 0 && e < a.n_pages) page = e;
+                    if (e >= 0 && e < a.n_pages) place = e * maps.kv.page_step + w.p.head * maps.kv.head_step;
                     else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
                 }
                 for (int kv = 0; ok && kv < 2; ++kv, ++it) {
@@ -195,8 +194,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                         if (ok) mbar_expect_tx(&full[s], C::OP);
                     }
                     ok = __shfl_sync(~0u, ok, 0);
-                    if (ok && lane < boxes)
-                        tma_load_4d(ring + s * C::OP + dst, kv ? &maps.v : &maps.k, half * 64, w.p.head, pos % a.page_size, page, &full[s]);
+                    if (ok && lane < pages)
+                        tma_load_5d(ring + s * C::OP + lane * rows * D * 2, kv ? &maps.kv.v : &maps.kv.k, pos % a.page_size / 8, place, &full[s]);
                 }
             }
             ++item;
@@ -213,19 +212,19 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             auto wait = [&](uint64_t *b, int parity) { return __all_sync(~0u, mbar_wait(b, parity, abort_flag, a.err)) != 0; };
             auto wait_slot = [&](int step) { return wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1); };
             auto scores = [&](int t, int step) {
-                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_k(ring + uniform(step % C::SLOTS) * C::OP);
+                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), 16, D * 16);
                 if (elect()) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t o = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4);
-                        tc::mma_ss(tb + t * 128, dq + o, dk + o, IDS, k != 0);
+                        const uint64_t oq = (uint64_t)((k / 4 * C::HALF + k % 4 * 32) >> 4), ok = (uint64_t)((k / 4 * 1024 + k % 4 * 32) >> 4);
+                        tc::mma_ss(tb + t * 128, dq + oq, dk + ok, IDS, k != 0);
                     }
                     tc::commit(&sfull[t]);
                 }
                 __syncwarp();
             };
             auto values = [&](int t, int step, bool first) {
-                const uint64_t dv = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), C::HALF, 1024);
+                const uint64_t dv = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), 1024, D * 16);
                 // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     if (elect()) {
 #pragma unroll
                         for (int k = h * 4; k < h * 4 + 4; ++k)
-                            tc::mma_ts(tb + 256 + t * 128, tb + t * 128 + k * 8, dv + (uint64_t)(k * 2048 >> 4), IDO, !(first && k == 0));
+                            tc::mma_ts(tb + 256 + t * 128, tb + t * 128 + k * 8, dv + (uint64_t)(k * D * 32 >> 4), IDO, !(first && k == 0));
                         if (h == 1) tc::commit(&pvdone[t]);
                     }
                     __syncwarp();
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     const int r0 = max(w.kv - p0, 0);
                     for (int e = i; e < (kLongUnit - r0) * (D / 8); e += 128) {
                         const int r = r0 + e / (D / 8), ch = e % (D / 8);
-                        *reinterpret_cast<uint4 *>(ring + s * C::OP + (ch >> 3) * C::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(ring + s * C::OP + kv_offset<D>(r, ch)) = make_uint4(0, 0, 0, 0);
                     }
                     tc::fence_proxy_async();
                     __syncwarp();
@@ -445,11 +444,10 @@ bool q_map(CUtensorMap *m, const AttendArgs &a, int d) {
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvMaps &kv, const AttendArgs &a, int parts, cudaStream_t s) {
+cudaError_t launch(const PoolMap &kv, const AttendArgs &a, int parts, cudaStream_t s) {
     LongMaps maps;
     std::memset(&maps, 0, sizeof(maps));
-    maps.k = kv.k;
-    maps.v = kv.v;
+    maps.kv = kv;
     if (!q_map(&maps.q, a, D)) return cudaErrorInvalidValue;
     using C = LongCfg<D>;
     cudaError_t e = dev::smem(attend_long_kernel<T, D>, C::SMEM);
@@ -459,7 +457,7 @@ cudaError_t launch(const KvMaps &kv, const AttendArgs &a, int parts, cudaStream_
 
 }  // namespace
 
-cudaError_t attend_long(const KvMaps &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s) {
+cudaError_t attend_long(const PoolMap &kv, const AttendArgs &a, bool bf16, int head_dim, int parts, cudaStream_t s) {
     if (head_dim == 64) return bf16 ? launch<__nv_bfloat16, 64>(kv, a, parts, s) : launch<__half, 64>(kv, a, parts, s);
     return bf16 ? launch<__nv_bfloat16, 128>(kv, a, parts, s) : launch<__half, 128>(kv, a, parts, s);
 }

@@ -61,6 +61,17 @@ inline bool nested(int64_t row, Axis a, Axis b, Axis c) {
     return true;
 }
 
+// The greatest step (elements) that reaches every page and head.
+inline int64_t pool_unit(const kg_pool &p) {
+    int64_t a = p.n_pages > 1 ? p.page_stride : 0, b = p.n_kv_head > 1 ? p.head_stride : 0;
+    while (b) {
+        const int64_t t = a % b;
+        a = b;
+        b = t;
+    }
+    return a ? a : p.head_dim;
+}
+
 inline int check_pool(kg_ctx *ctx, const kg_pool *p) {
     if (!p) return fail(ctx, KG_ERR_INVALID_ARG, "null pool");
     if (!p->k || !p->v || p->k == p->v) return fail(ctx, KG_ERR_INVALID_ARG, "pool: k and v must be two device pointers");
@@ -77,6 +88,9 @@ inline int check_pool(kg_ctx *ctx, const kg_pool *p) {
     if (p->page_stride < 0 || p->row_stride < 0 || p->head_stride < 0 ||
         !nested(p->head_dim, {p->page_stride, p->n_pages}, {p->row_stride, p->page_size}, {p->head_stride, p->n_kv_head}))
         return fail(ctx, KG_ERR_INVALID_ARG, "pool: rows overlap at these strides");
+    const int64_t span = (p->n_pages > 1 ? (p->n_pages - 1) * p->page_stride : 0) + (p->n_kv_head > 1 ? (p->n_kv_head - 1) * p->head_stride : 0);
+    if (span / pool_unit(*p) >= INT32_MAX || p->row_stride >= (int64_t)1 << 35)
+        return fail(ctx, KG_ERR_UNSUPPORTED, "pool: page and head strides with a larger common divisor are needed for this many pages");
     return KG_OK;
 }
 
