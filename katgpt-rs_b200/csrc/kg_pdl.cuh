@@ -13,6 +13,10 @@ namespace kg {
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
+// Lets the next kernel of the stream start once every CTA has come here or ended; that kernel may then not wait
+// (pdl_wait) before it needs this one's results.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
 // kernel<<<grid, block, smem, s>>>(args...) with the programmatic-serialization
 // attribute, as thread-block clusters of `cluster` when it is not 1 x 1 x 1.
 template <typename... KArgs, typename... Args>

@@ -70,7 +70,8 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ PoolMap maps, const AttendArgs a) {
+__global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ PoolMap maps, const AttendArgs a,
+                                                                   int after_long) {
     using C = ShortCfg<D>;
     extern __shared__ __align__(1024) uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (sa(raw) & 1023u)) & 1023u);
@@ -88,13 +89,18 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
         *abort_flag = 0;
         mbar_fence_init();
     }
-    pdl_wait();
+    // Behind the long requests' kernel this one starts as soon as that one's CTAs all run (they have waited for what came
+    // before), and waits for it at its own end: the two share the device, and what follows waits for both.
+    if (!after_long) pdl_wait();
     int req;
     long long off, units;
     find_part<SHORT_THREADS, false>(a, c, gridDim.x, SHORT_LEAST, part_sm, req, off, units);  // (synchronises)
     if (threadIdx.x < 2) a.meta[2 * c + threadIdx.x].x = 0;
     __syncthreads();
-    if (units == 0) return;
+    if (units == 0) {
+        if (after_long) pdl_wait();
+        return;
+    }
     Walk<false> w;
     w.start(a, req, off, units);
 
@@ -120,12 +126,14 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                 }
                 if (!__shfl_sync(~0u, ok, 0)) {
                     drain_loads(full, C::STAGES, it);
+                    if (after_long) pdl_wait();
                     return;
                 }
                 if (lane < boxes)
                     tma_load_5d(sm + s * 2 * C::OP_BYTES + dst, tm, pos % a.page_size / 8, place, &full[s]);
             }
         } while (w.next(a));
+        if (after_long) pdl_wait();
         return;
     }
 
@@ -288,43 +296,53 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
         }
         if (!whole && threadIdx.x == 0) a.meta[slot] = make_int4(w.ends() ? 3 : 1, w.r, w.p.head, 0);
     } while (w.next(a));
+    if (after_long) pdl_wait();
 }
 
-// Joins the parts of an item that was cut: CTA c looks after the item that
-// begins in part c and ends beyond it. Part sums are added in the order of the
-// parts, so results do not depend on timing.
-template <typename T, int D, bool LONG>
-__global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, int parts) {
+// Joins the parts of the items that were cut, of both kernels: block x looks after
+// the item that begins in part x and ends beyond it, eight rows a block in turn.
+// Few parts: a warp a row; many (a lone long sequence): the block's warps share a
+// row's parts. Part sums are added in a fixed order, so results do not depend on
+// timing.
+constexpr int JOIN_ROWS = 8, JOIN_FEW = 16;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, int short_parts, const AttendArgs lo) {
     pdl_wait();
     __shared__ int s_last;
     __shared__ float4 sums[8][32];
     __shared__ float part_l[8];
-    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool is_long = (int)blockIdx.x >= short_parts;
+    const AttendArgs &a = is_long ? lo : sh;
+    const int c = is_long ? blockIdx.x - short_parts : blockIdx.x, parts = is_long ? gridDim.x - short_parts : short_parts;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int4 me = a.meta[2 * c + 1];
     if (me.x == 0) return;
+    int q0, q, kv;
+    req_len(a, me.y, q0, q, kv);
+    const int group = a.s.group, tq = a.s.tile / 2, rows = is_long ? 256 : q * group;
+    if ((int)blockIdx.y * JOIN_ROWS >= rows) return;
     if (threadIdx.x == 0) {
         int e = c + 1;
         while (e < parts - 1 && a.meta[2 * e].x == 1) ++e;
         s_last = e;
     }
     __syncthreads();
-    int q0, q, kv;
-    req_len(a, me.y, q0, q, kv);
-    const int n = s_last - c + 1, group = a.s.group, tq = a.s.tile / 2;
-    const int rows = LONG ? 256 : q * group;
+    const int n = s_last - c + 1;
     auto slot = [&](int i) { return a.part + (i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.slot_floats; };
     constexpr int PER = D / 32;  // dims of a lane
-    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-        const int i = LONG ? row & 127 : row;
-        const int tok = LONG ? (me.w * 2 + (row >> 7)) * tq + i / group : i / group;
-        if (LONG && (i >= tq * group || tok >= q)) continue;
+    auto each = [&](int r) {     // row r of this block: token, or -1
+        const int row = blockIdx.y * JOIN_ROWS + r, i = is_long ? row & 127 : row;
+        const int tok = is_long ? (me.w * 2 + (row >> 7)) * tq + i / group : i / group;
+        return row >= rows || (is_long && i >= tq * group) || tok >= q ? -1 : tok;
+    };
+    auto sum_of = [&](int row, int first, int step, float (&o)[PER], float &l) {
         auto stat_of = [&](int k) { return reinterpret_cast<const float2 *>(slot(k) + (int64_t)a.rows * D)[row]; };
         float top = -INFINITY;
         for (int k = lane; k < n; k += 32) top = fmaxf(top, stat_of(k).x);
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        float o[PER] = {}, l = 0.0f;
 #pragma unroll 4
-        for (int k = warp; k < n; k += 8) {
+        for (int k = first; k < n; k += step) {
             const float2 s = stat_of(k);
             if (s.x == -INFINITY) continue;  // nothing was attended there, nothing was written
             const float f = exp2_approx(s.x - top);
@@ -333,21 +351,43 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs a, in
 #pragma unroll
             for (int e = 0; e < PER; ++e) o[e] += p[e] * f;
         }
+    };
+    auto write = [&](int row, int tok, const float (&o)[PER], float l) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const int i = is_long ? row & 127 : row;
+        T *dst = static_cast<T *>(a.out) + (int64_t)(q0 + tok) * a.o_row + (me.z * group + i % group) * a.o_head + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t *>(dst)[e / 2] = Cvt<T>::pack(o[e] * inv, o[e + 1] * inv);
+    };
+    if (n <= JOIN_FEW) {
+        const int tok = each(warp), row = blockIdx.y * JOIN_ROWS + warp;
+        if (tok < 0) return;
+        float o[PER] = {}, l = 0.0f;
+        sum_of(row, 0, 1, o, l);
+        write(row, tok, o, l);
+        return;
+    }
+    for (int r = 0; r < JOIN_ROWS; ++r) {
+        const int tok = each(r), row = blockIdx.y * JOIN_ROWS + r;
+        if (tok < 0) continue;
+        float o[PER] = {}, l = 0.0f;
+        sum_of(row, warp, 8, o, l);
         sums[warp][lane] = make_float4(o[0], o[1], PER > 2 ? o[PER - 2] : 0.0f, PER > 2 ? o[PER - 1] : 0.0f);
         if (lane == 0) part_l[warp] = l;
         __syncthreads();
         if (warp == 0) {
-            float4 t = make_float4(0, 0, 0, 0);
-            float total = 0.0f;
+            float t[PER] = {}, total = 0.0f;
             for (int k = 0; k < 8; ++k) {
                 const float4 x = sums[k][lane];
-                t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+                t[0] += x.x;
+                t[1] += x.y;
+                if (PER > 2) {
+                    t[PER - 2] += x.z;
+                    t[PER - 1] += x.w;
+                }
                 total += part_l[k];
             }
-            const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-            T *dst = static_cast<T *>(a.out) + (int64_t)(q0 + tok) * a.o_row + (me.z * group + i % group) * a.o_head + lane * PER;
-            reinterpret_cast<uint32_t *>(dst)[0] = Cvt<T>::pack(t.x * inv, t.y * inv);
-            if (PER > 2) reinterpret_cast<uint32_t *>(dst)[1] = Cvt<T>::pack(t.z * inv, t.w * inv);
+            write(row, tok, t, total);
         }
         __syncthreads();
     }
@@ -370,7 +410,7 @@ bool pool_map(PoolMap &m, const kg_pool &p) {
     const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     for (int i = 0; i < 2; ++i)
         if (fn(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, i ? p.v : p.k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return false;
     return true;
 }
@@ -403,24 +443,25 @@ cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *worksp
     cudaError_t e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
     if (e != cudaSuccess) return e;
     const int parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
+    AttendArgs b = a;
+    int long_parts = 0;
     if (sp.may_long) {
-        AttendArgs b = a;
         b.meta = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + sp.long_at);
         b.part = reinterpret_cast<float *>(b.meta + 2 * kMaxLongParts);
         b.slot_floats = sp.long_floats;
         b.rows = 256;
-        const int long_parts = std::min(kMaxLongParts, dev::sm_count());
+        long_parts = std::min(kMaxLongParts, dev::sm_count());
         e = attend_long(maps, b, std::is_same<T, __nv_bfloat16>::value, D, long_parts, s);
-        if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D, true>, dim3(long_parts, 32), dim3(256), 0, s, b, long_parts);
         if (e != cudaSuccess) return e;
     }
     a.meta = static_cast<int4 *>(workspace);
     a.part = reinterpret_cast<float *>(a.meta + 2 * kMaxParts);
     a.slot_floats = sp.slot_floats;
     a.rows = sp.rows;
-    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a);
-    if (e == cudaSuccess) e = launch_pdl(attend_join_kernel<T, D, false>, dim3(parts, std::min(a.rows, 16)), dim3(256), 0, s, a, parts);
-    return e;
+    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a, (int)sp.may_long);
+    if (e != cudaSuccess) return e;
+    const int rows = sp.may_long ? 256 : a.rows;
+    return launch_pdl(attend_join_kernel<T, D>, dim3(parts + long_parts, (rows + JOIN_ROWS - 1) / JOIN_ROWS), dim3(256), 0, s, a, parts, b);
 }
 
 int check(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q) {

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         mbar_fence_init();
     }
     pdl_wait();
+    pdl_launch();  // the short requests' kernel may take the SMs that this one leaves free
     int req;
     long long off, units;
     find_part<LONG_THREADS, true>(a, c, gridDim.x, LONG_LEAST, part_sm, req, off, units);
