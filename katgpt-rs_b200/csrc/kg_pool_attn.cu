@@ -258,21 +258,24 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
         const bool whole = w.whole();
         const int slot = 2 * c + w.slot();
         float *part = a.part + slot * a.slot_floats;
-        for (int d0 = 0; d0 < D; d0 += 32) {
-            float *mine = scratch + warp * 16 * 36;
+        // `width` dims of every row at a time, as the scratch holds: all of them where a request has few rows
+        const int few = rows <= 4, width = few ? D : 32, pitch = few ? D : 36, cap = few ? 4 : 16;
+        for (int d0 = 0; d0 < D; d0 += width) {
+            float *mine = scratch + warp * cap * pitch;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
-                if (n / 4 == d0 / 32)
+                if (few || n / 4 == d0 / 32)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        *reinterpret_cast<float2 *>(mine + (gid + 8 * i) * 36 + (n & 3) * 8 + tig * 2) =
-                            make_float2(o[n][i * 2] * f[i], o[n][i * 2 + 1] * f[i]);
+                        if (gid + 8 * i < cap)
+                            *reinterpret_cast<float2 *>(mine + (gid + 8 * i) * pitch + (few ? n : n & 3) * 8 + tig * 2) =
+                                make_float2(o[n][i * 2] * f[i], o[n][i * 2 + 1] * f[i]);
             bar_consumers();
-            for (int i = threadIdx.x; i < rows * 8; i += 128) {
-                const int row = i >> 3, d = (i & 7) * 4, g = row >> 4, r = row & 15;
+            for (int i = threadIdx.x; i < rows * (width / 4); i += 128) {
+                const int row = few ? i / (D / 4) : i >> 3, d = (few ? i % (D / 4) : i & 7) * 4, g = row >> 4, r = row & 15;
                 float4 sum = make_float4(0, 0, 0, 0);
                 for (int k = g; k < 4; k += wm) {
-                    const float4 x = *reinterpret_cast<const float4 *>(scratch + (k * 16 + r) * 36 + d);
+                    const float4 x = *reinterpret_cast<const float4 *>(scratch + (k * cap + r) * pitch + d);
                     sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
                 }
                 const float top = top_of(g, r);
@@ -410,7 +413,8 @@ bool pool_map(PoolMap &m, const kg_pool &p) {
     const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     for (int i = 0; i < 2; ++i)
         if (fn(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, i ? p.v : p.k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+               CU_TENSOR_MAP_SWIZZLE_128B, p.head_dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return false;
     return true;
 }

@@ -62,8 +62,14 @@ KG_HD int64_t long_units_of_head(const Shape &s, int q, int kv) {
 KG_HD int64_t request_units(const Shape &s, bool is_long, int q, int kv) {
     return (is_long ? long_units_of_head(s, q, kv) : short_units(s, q, kv)) * s.n_kv;
 }
-// the first unit of part c of `parts`
-KG_HD int64_t part_begin(int64_t units, int c, int parts) { return units / parts * c + units % parts * c / parts; }
+// the first unit of part c of `parts` (in 32 bits where they suffice: 64-bit divisions are slow on the device)
+KG_HD int64_t part_begin(int64_t units, int c, int parts) {
+    if (units <= 4194303) {  // units % parts * c stays below 512 * 512
+        const uint32_t n = (uint32_t)units, p = (uint32_t)parts, k = (uint32_t)c;
+        return n / p * k + n % p * k / p;
+    }
+    return units / parts * c + units % parts * c / parts;
+}
 
 // A place in the line: item (head, tile) of a request, its first unit here and its length.
 struct Place {
@@ -73,8 +79,13 @@ KG_HD Place place_of(const Shape &s, bool is_long, int q, int kv, int64_t off) {
     Place p;
     if (!is_long) {
         p.units = short_units(s, q, kv);
-        p.head = (int)(off / p.units);
-        p.unit = (int)(off % p.units);
+        if (off <= 0x7fffffff) {
+            p.head = (int)((uint32_t)off / (uint32_t)p.units);
+            p.unit = (int)((uint32_t)off % (uint32_t)p.units);
+        } else {
+            p.head = (int)(off / p.units);
+            p.unit = (int)(off % p.units);
+        }
         p.tile = 0;
         return p;
     }
