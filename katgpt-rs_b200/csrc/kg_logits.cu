@@ -10,15 +10,18 @@
 // index below the cut's.
 //
 // A row is held in the shared memory of a cluster of 1 to 8 CTAs and read from
-// global memory once. A histogram of (max - x) / T in steps of 1/64 says where the
-// cuts must lie:
-//   - where the candidates down to that step are at most 512 (small top-k, a peaked
-//     row), they go to the cluster's first CTA, which ranks and cuts them alone;
-//   - else the tokens of the step (top-k) or of three steps (top-p) that hold the cut
-//     go there, at most 4096, and the cut is found by bisection of their keys against
-//     the exact sum above them; the token is drawn by all CTAs;
-//   - where that does not hold (rows of equal values), by bisection over the row.
-// Weights cost about 12 operations in 64 bits: they are computed for what a sum needs.
+// global memory once. A histogram of (max - x) / T in steps of 1/64, of entries and
+// for top-p of weights, says in which step each cut lies (each CTA adds up its share
+// of the steps):
+//   - where the candidates down to that step are at most 2048 (small top-k, a peaked
+//     row), they go to the cluster's first CTA, which finishes the row alone: it ranks
+//     up to 128 of them in both orders, or bisects their keys and indexes;
+//   - else the entries of that one step go there and the cut is bisected against the
+//     sum above them; the token is drawn by all CTAs;
+//   - where a step holds more than 2048 (rows of equal values), by bisection over the
+//     whole row.
+// Weights cost about 14 operations in 64 bits, which run at a half of the 32-bit
+// rate: they are computed once for top-p's histogram and once for what is drawn from.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -61,8 +64,8 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, LOCAL = 512, LIST = 4096;
-static_assert(LOCAL == THREADS, "a thread has one candidate");
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, RANKED = 128, LIST = 2048;
+constexpr int PER = LIST / THREADS;  // candidates of a thread
 
 // ---- cluster
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -89,6 +92,7 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t a) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ int pack_bits(u64 v, int at, int bits) { return (int)(v >> at & ((1ull << bits) - 1)); }
 __device__ __forceinline__ u64 remote_u64(uint32_t a) {
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
@@ -102,17 +106,20 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t a, uint32_t v) {
 }
 
 struct Shared {
-    double tab[64];        // 2^(j / 64)
-    u64 warp[2][WARPS];    // block sums
-    u64 red[2];            // this CTA's part of a cluster sum
-    u64 cut;               // (key << 32 | index) found by the first CTA
-    uint32_t n_list, wanted[2];
-    int32_t found;
+    double tab[64];      // 2^(j / 64)
+    u64 warp[2][WARPS];  // block sums
+    u64 red[2][3];       // this CTA's part of what a cluster shares
+    uint32_t n_list;
+    uint32_t queue[WARPS][64];
     union {
         struct {
-            uint32_t hist[BINS], sum[BINS];  // this CTA's counts, the cluster's
+            uint32_t count[BINS], low[BINS], high[BINS];  // entries and weights (two words) of this CTA's slice by step
         };
-        u64 list[LIST];  // key << 32 | index, of the first CTA
+        struct {
+            u64 list[LIST];  // key << 32 | index, of the first CTA
+            u64 order[RANKED];
+            uint32_t place[RANKED], index[RANKED];
+        };
     };
 };
 
@@ -145,10 +152,11 @@ struct Weigh {
     __device__ __forceinline__ u64 operator()(uint32_t k) const { return k ? whole(real(k)) : 0ull; }
 };
 
+// sum over the warp, below 2^63: three parts of 26 bits whose sums stay in 32
 __device__ __forceinline__ u64 warp_sum(u64 v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-    return v;
+    const uint32_t a = __reduce_add_sync(~0u, (uint32_t)v & 0x3ffffffu), b = __reduce_add_sync(~0u, (uint32_t)(v >> 26) & 0x3ffffffu),
+                   c = __reduce_add_sync(~0u, (uint32_t)(v >> 52));
+    return (u64)a + ((u64)b << 26) + ((u64)c << 52);
 }
 
 template <typename T>
@@ -177,11 +185,42 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         return warp_sum(v);
     };
     int turn = 0;
-    // every CTA's v (the same in all its threads): f(rank, v)
-    auto gather = [&](u64 v, auto f) {
-        if (tid == 0) sh.red[turn & 1] = v;
+    // every CTA's values (v, x, y: the same in all its threads, or those of the thread that names them by `mine`): f(rank, v, x, y)
+    auto share = [&](bool mine, u64 v, u64 x, u64 y, auto f) {
+        u64 *to = sh.red[turn & 1];
+        if (mine) {
+            to[0] = v;
+            to[1] = x;
+            to[2] = y;
+        }
+        __syncwarp();
         cluster_sync();
-        for (uint32_t r = 0; r < C; ++r) f(r, remote_u64(remote(&sh.red[turn & 1], r)));
+        u64 got[8][3];
+#pragma unroll
+        for (uint32_t r = 0; r < 8; ++r)
+            if (r < C) {
+                const uint32_t at = remote(to, r);
+                got[r][0] = remote_u64(at);
+                got[r][1] = remote_u64(at + 8);
+                got[r][2] = remote_u64(at + 16);
+            }
+#pragma unroll
+        for (uint32_t r = 0; r < 8; ++r)
+            if (r < C) f(r, got[r][0], got[r][1], got[r][2]);
+        ++turn;
+    };
+    auto gather = [&](u64 v, auto f) {
+        u64 *to = sh.red[turn & 1];
+        if (tid == 0) to[0] = v;
+        __syncwarp();
+        cluster_sync();
+        u64 got[8];
+#pragma unroll
+        for (uint32_t r = 0; r < 8; ++r)
+            if (r < C) got[r] = remote_u64(remote(to, r));
+#pragma unroll
+        for (uint32_t r = 0; r < 8; ++r)
+            if (r < C) f(r, got[r]);
         ++turn;
     };
     auto cluster_sum = [&](u64 v) {
@@ -274,108 +313,169 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         ck = c;
         ci = hi;
     };
-    // The same over the first CTA's list; the cut goes to every CTA.
-    auto cut_list = [&](u64 want, auto f, auto per_equal) {
-        if (rank == 0) {
-            const int m = (int)sh.n_list;
-            auto sum = [&](auto g) {
-                u64 s = 0;
-                for (int i = tid; i < m; i += THREADS) {
-                    const u64 e = sh.list[i];
-                    s += g((uint32_t)(e >> 32), (uint32_t)e);
-                }
-                return block_sum(s);
-            };
-            uint32_t lo = 0, hi = 0;  // keys that the list's share the leading bits of
-            {
-                uint32_t x = 0, y = ~0u;
-                for (int i = tid; i < m; i += THREADS) {
-                    const uint32_t k = (uint32_t)(sh.list[i] >> 32);
-                    x = max(x, k);
-                    y = min(y, k);
-                }
-                x = __reduce_max_sync(~0u, x);
-                y = __reduce_min_sync(~0u, y);
-                u64 *w = sh.warp[flip & 1];
-                ++flip;
-                if (lane == 0) w[warp] = (u64)x << 32 | y;
-                __syncthreads();
-                hi = __reduce_max_sync(~0u, lane < WARPS ? (uint32_t)(w[lane] >> 32) : 0u);
-                lo = __reduce_min_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : ~0u);
-            }
-            while (lo < hi) {  // sum(>= lo) reaches want; the cut is in [lo, hi]
-                const uint32_t mid = lo + (hi - lo + 1) / 2;
-                if (sum([&](uint32_t k, uint32_t j) { return k >= mid ? f(k, j) : 0ull; }) >= want) lo = mid;
-                else hi = mid - 1;
-            }
-            const uint32_t c = lo;
-            const u64 above = sum([&](uint32_t k, uint32_t j) { return k > c ? f(k, j) : 0ull; });
-            const u64 w = per_equal(c), take = (want - above + w - 1) / w;
-            const u64 have = sum([&](uint32_t k, uint32_t j) { return k == c && stays(k, j) ? 1ull : 0ull; });
-            uint32_t at = ~0u;  // all of the equals
-            if (take < have) {
-                uint32_t l = 0;
-                at = a.vocab;
-                while (at - l > 1) {
-                    const uint32_t mid = (l + at) / 2;
-                    if (sum([&](uint32_t k, uint32_t j) { return k == c && j < mid && stays(k, j) ? 1ull : 0ull; }) >= take) at = mid;
-                    else l = mid;
-                }
-            }
-            if (tid == 0) sh.cut = (u64)c << 32 | at;
+    // The first CTA's list, PER entries a thread in registers, and cuts of it: in the first CTA only.
+    uint32_t lk[PER], lj[PER];
+    u64 lw[PER];
+    auto list_load = [&](bool weights) {
+        const int m = (int)sh.n_list;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int i = tid + e * THREADS;
+            const u64 x = i < m ? sh.list[i] : 0ull;
+            lk[e] = (uint32_t)(x >> 32);
+            lj[e] = (uint32_t)x;
+            lw[e] = weights ? weigh(lk[e]) : lk[e] ? 1ull : 0ull;
         }
-        cluster_sync();
-        const u64 x = remote_u64(remote(&sh.cut, 0));
-        const uint32_t ci_before = ci, ck_before = ck;
+    };
+    auto list_sum = [&](auto f) {
+        u64 s = 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) s += f(lk[e], lj[e], lw[e]);
+        return block_sum(s);
+    };
+    // the cut of the entries that stay at the first place where the sum of lw reaches `want`
+    auto list_cut = [&](u64 want, bool weights) {
+        uint32_t x = 0, y = ~0u;
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (lk[e]) {
+                x = max(x, lk[e]);
+                y = min(y, lk[e]);
+            }
+        x = __reduce_max_sync(~0u, x);
+        y = __reduce_min_sync(~0u, y);
+        u64 *w = sh.warp[flip & 1];
+        ++flip;
+        if (lane == 0) w[warp] = (u64)x << 32 | y;
+        __syncthreads();
+        uint32_t hi = __reduce_max_sync(~0u, lane < WARPS ? (uint32_t)(w[lane] >> 32) : 0u);
+        uint32_t lo = __reduce_min_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : ~0u);
+        u64 above = 0;
+        while (lo < hi) {  // the sum over keys >= lo reaches want, that over keys > hi, `above`, does not
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            const u64 s = list_sum([&](uint32_t k, uint32_t j, u64 v) { return k >= mid && stays(k, j) ? v : 0ull; });
+            if (s >= want) {
+                lo = mid;
+            } else {
+                hi = mid - 1;
+                above = s;
+            }
+        }
+        const uint32_t c = lo;
+        const u64 each = weights ? weigh(c) : 1ull, take = (want - above + each - 1) / each;
+        const u64 have = list_sum([&](uint32_t k, uint32_t j, u64) { return k == c && stays(k, j) ? 1ull : 0ull; });
+        uint32_t at = ck == c ? ci : ~0u;  // all of the equals that stay
+        if (take < have) {
+            uint32_t l = 0;
+            at = a.vocab;
+            while (at - l > 1) {
+                const uint32_t mid = (l + at) / 2;
+                if (list_sum([&](uint32_t k, uint32_t j, u64) { return k == c && j < mid && stays(k, j) ? 1ull : 0ull; }) >= take) at = mid;
+                else l = mid;
+            }
+        }
+        ck = c;
+        ci = at;
+    };
+    // the same, for every CTA
+    auto cut_list = [&](u64 want, bool weights) {
+        if (rank == 0) {
+            list_load(weights);
+            list_cut(want, weights);
+        }
+        u64 x = 0;
+        gather((u64)ck << 32 | ci, [&](uint32_t r, u64 v) { x = r == 0 ? v : x; });
         ck = (uint32_t)(x >> 32);
         ci = (uint32_t)x;
-        if (ck == ck_before) ci = min(ci, ci_before);
     };
-    // live entries whose bin is in [b0, b1] into the first CTA's list (only what stays)
+    // live entries whose bin is in [b0, b1] and that stay, into the first CTA's list
     auto to_list = [&](int b0, int b1) {
-        if (tid == 0) sh.n_list = 0;
-        cluster_sync();  // (and the histograms, which lie under the list, have been read)
-        const uint32_t count = remote(&sh.n_list, 0), dst = remote(sh.list, 0);
-        for (int i0 = 0; i0 < n; i0 += THREADS) {
-            const int i = i0 + tid;
-            const uint32_t k = i < n ? keys[i] : 0u;
-            bool in = k != 0;
-            if (in) {
-                const int b = bin_of(k);
-                in = b >= b0 && b <= b1 && stays(k, (uint32_t)(base + i));
-            }
-            const uint32_t who = __ballot_sync(~0u, in);
-            if (who == 0) continue;
-            uint32_t at = 0;
-            if (lane == __ffs(who) - 1) at = remote_add(count, __popc(who));
-            at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-            if (in && at < LIST) remote_store(dst + at * 8, (u64)k << 32 | (uint32_t)(base + i));
+        u64 in = 0;  // of this thread's entries
+        for (int i = tid, e = 0; i < n; i += THREADS, ++e) {
+            const uint32_t k = keys[i];
+            if (k == 0) continue;
+            const int b = bin_of(k);
+            if (b >= b0 && b <= b1 && stays(k, (uint32_t)(base + i))) in |= 1ull << e;
         }
+        if (tid == 0) sh.n_list = 0;
+        cluster_sync();  // (the histograms, which lie under the list, have been read)
+        const uint32_t mine = __popcll(in);
+        uint32_t x = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
+        }
+        uint32_t at = 0;
+        if (lane == 31 && x) at = remote_add(remote(&sh.n_list, 0), x);
+        at = __shfl_sync(~0u, at, 31) + x - mine;
+        const uint32_t dst = remote(sh.list, 0);
+        for (; in; in &= in - 1, ++at)
+            if (at < LIST) {
+                const int i = tid + (__ffsll((long long)in) - 1) * THREADS;
+                remote_store(dst + at * 8, (u64)keys[i] << 32 | (uint32_t)(base + i));
+            }
+        __syncwarp();
         cluster_sync();
+    };
+    auto pick = [&](u64 K) {  // the place in the running sum that the given number names
+        const double uu = u_in > 0.0f ? (double)u_in : 0.0;
+        const u64 t = uu >= 1.0 ? K - 1 : (u64)(uu * (double)K);
+        return t > K - 1 ? K - 1 : t;
+    };
+    auto part_of = [&](u64 W) {  // what top-p has to reach
+        const double t = ceil((double)fmaxf(p, 0.0f) * (double)W);
+        return t < 1.0 ? 1ull : (u64)t;
     };
 
     const u64 kk = want_k > 0 && want_k < a.vocab ? (u64)want_k : 0ull;
-    if (kk || p < 1.0f) {
-        // counts by bin, and where no top-k precedes it the whole sum for top-p
-        for (int i = tid; i < BINS; i += THREADS) sh.hist[i] = 0;
+    const bool has_p = p < 1.0f;
+    if (kk || has_p) {
+        for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.low[i] = sh.high[i] = 0;
         __syncthreads();
-        u64 mine = 0;
-        const bool mass = p < 1.0f && !kk;
         for (int i = tid; i < n; i += THREADS) {
             const uint32_t k = keys[i];
             if (k == 0) continue;
-            atomicAdd(&sh.hist[bin_of(k)], 1u);
-            if (mass) mine += weigh(k);
+            const int b = bin_of(k);
+            atomicAdd(&sh.count[b], 1u);
+            if (has_p) {
+                const u64 w = weigh(k);
+                const uint32_t lo = (uint32_t)w;
+                uint32_t hi = (uint32_t)(w >> 32);
+                if (lo && atomicAdd(&sh.low[b], lo) > ~lo) ++hi;
+                if (hi) atomicAdd(&sh.high[b], hi);
+            }
         }
-        u64 W = cluster_sum(mine);  // (synchronises: every histogram is complete)
-        uint32_t cnt[BINS / THREADS];
-        const int b0 = tid * (BINS / THREADS);
-        for (int j = 0; j < BINS / THREADS; ++j) cnt[j] = 0;
-        for (uint32_t r = 0; r < C; ++r) {
-            const uint32_t h = remote(&sh.hist[b0], r);
-            for (int j = 0; j < BINS / THREADS; ++j) cnt[j] += remote_u32(h + j * 4);
+        __syncwarp();
+        cluster_sync();
+        // this CTA's share of the steps: entries and weights of the whole row
+        const int share_bins = BINS / (int)C, nb = max(1, share_bins / THREADS);
+        const bool owner = tid * nb < share_bins;
+        const int first = (int)rank * share_bins + tid * nb;
+        u64 c[4], w[4], c_all = 0, w_all = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c[j] = w[j] = 0;
+            if (owner && j < nb) {
+                uint32_t x[8], y[8], z[8];
+                const int b = first + j;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r)
+                    if (r < C) {
+                        x[r] = remote_u32(remote(&sh.count[b], r));
+                        y[r] = has_p ? remote_u32(remote(&sh.low[b], r)) : 0u;
+                        z[r] = has_p ? remote_u32(remote(&sh.high[b], r)) : 0u;
+                    }
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r)
+                    if (r < C) {
+                        c[j] += x[r];
+                        w[j] += ((u64)z[r] << 32) + y[r];
+                    }
+            }
+            c_all += c[j];
+            w_all += w[j];
         }
-        // running sums of counts and of estimated weights over the bins
         auto scan = [&](u64 v) {  // exclusive, over the block's threads
             u64 x = v;
 #pragma unroll
@@ -383,147 +483,186 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
                 const u64 y = __shfl_up_sync(~0u, x, d);
                 if (lane >= d) x += y;
             }
-            u64 *w = sh.warp[flip & 1];
+            u64 *to = sh.warp[flip & 1];
             ++flip;
-            if (lane == 31) w[warp] = x;
+            if (lane == 31) to[warp] = x;
             __syncthreads();
             u64 before = 0;
-            for (int k = 0; k < warp; ++k) before += w[k];
+            for (int k = 0; k < warp; ++k) before += to[k];
             return before + x - v;
         };
-        u64 c_here = 0, e_here = 0;
-        auto guess = [&](int b) { return (u64)(exp2f((b + 0.5f) * (-1.44269504f / 64.0f)) * 1073741824.0f) + 1; };
-        for (int j = 0; j < BINS / THREADS; ++j) {
-            c_here += cnt[j];
-            e_here += cnt[j] * guess(b0 + j);
-        }
-        u64 c_run = scan(c_here), e_run = scan(e_here);
-        const u64 live = block_sum(c_here), e_all = block_sum(e_here);
+        u64 c_run = scan(c_all), w_run = has_p ? scan(w_all) : 0ull, live = 0, W = 0;
+        share(tid == THREADS - 1, c_run + c_all, w_run + w_all, 0, [&](uint32_t r, u64 x, u64 y, u64) {
+            if (r == rank) {
+                c_run += live;
+                w_run += W;
+            }
+            live += x;
+            W += y;
+        });
+        // The step that holds the k-th entry: {step, entries before it, entries in it}, 12, 20 and 20 bits and a mark.
+        auto packed = [&](int b, u64 before, u64 in) { return 1ull << 63 | (u64)b << 40 | before << 20 | in; };
         const bool use_k = kk && kk < live;
-        if (kk && !use_k && p < 1.0f) W = over([&](uint32_t k, uint32_t) { return weigh(k); });
-        // the bin of the k-th entry, the bin where top-p's cut is expected, and the counts down to them
-        const u64 e_want = (u64)((double)fmaxf(p, 0.0f) * (double)e_all);
-        if (tid == 0) sh.wanted[0] = sh.wanted[1] = BINS - 1;
-        __syncthreads();
-        for (int j = 0; j < BINS / THREADS; ++j) {
-            const u64 e = cnt[j] * guess(b0 + j);
-            if (use_k && c_run < kk && kk <= c_run + cnt[j]) sh.wanted[0] = b0 + j;
-            if (e_run <= e_want && e_want < e_run + e) sh.wanted[1] = b0 + j;
-            sh.sum[b0 + j] = (uint32_t)(c_run += cnt[j]);  // entries in bins <= b
-            e_run += e;
+        int bk = BINS, before_k = 0, n_k = 0;
+        if (use_k) {
+            u64 x = c_run, hit = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (owner && x < kk && kk <= x + c[j]) hit = packed(first + j, x, c[j]);
+                x += c[j];
+            }
+            if (tid == 0) sh.red[turn & 1][0] = 0;
+            __syncthreads();
+            u64 got = 0;
+            share(hit != 0, hit, 0, 0, [&](uint32_t, u64 v, u64, u64) { got = max(got, v); });
+            bk = pack_bits(got, 40, 12);
+            before_k = pack_bits(got, 20, 20);
+            n_k = pack_bits(got, 0, 20);
         }
-        __syncthreads();
-        const int bk = (int)sh.wanted[0], bp = (int)sh.wanted[1];
-        auto upto = [&](int b) { return b < 0 ? 0u : sh.sum[b]; };
-        const uint32_t n_local = upto(use_k ? bk : min(bp + 1, BINS - 1));
-        const uint32_t n_k = use_k ? upto(bk) - upto(bk - 1) : 0u;
-        const u64 k_left = use_k ? kk - upto(bk - 1) : 0ull;
-        const int p0 = max(bp - 1, 0), p1 = min(bp + 1, BINS - 1);
-        const uint32_t n_p = upto(p1) - upto(p0 - 1);
-        if (n_local <= LOCAL && (use_k || p < 1.0f)) {
-            // Few candidates: the first CTA ranks them in both orders and finishes the row.
-            to_list(0, use_k ? bk : p1);
+        // The step that holds the place where the weights reach `want` (among the first bk, or bk itself).
+        u64 above = 0;
+        int bp = BINS, before_p = 0, n_p = 0;
+        auto find_weight = [&](u64 want) {
+            u64 x = w_run, y = c_run, hit = 0, hit_above = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = first + j;
+                if (owner && j < nb && x < want && (b < bk ? want <= x + w[j] : b == bk)) {
+                    hit = packed(b, y, c[j]);
+                    hit_above = x;
+                }
+                x += w[j];
+                y += c[j];
+            }
+            if (tid == 0) sh.red[turn & 1][0] = 0;
+            __syncthreads();
+            u64 got = 0;
+            share(hit != 0, hit, hit_above, 0, [&](uint32_t, u64 v, u64 ab, u64) {
+                if (v) {
+                    got = v;
+                    above = ab;
+                }
+            });
+            bp = pack_bits(got, 40, 12);
+            before_p = pack_bits(got, 20, 20);
+            n_p = pack_bits(got, 0, 20);
+        };
+        if (!use_k && has_p) find_weight(part_of(W));
+        const int all_of = use_k ? before_k + n_k : before_p + n_p;
+        if ((use_k || has_p) && all_of <= LIST) {
+            // Few candidates: the first CTA finishes the row.
+            to_list(0, use_k ? bk : bp);
             if (rank == 0) {
-                const int m = (int)sh.n_list;
-                u64 *by_order = sh.list + LOCAL;                                      // weights in order
-                uint32_t *place = reinterpret_cast<uint32_t *>(sh.list + 2 * LOCAL);  // by index: place in the order, then the index
-                __syncthreads();
-                if (tid < m) {
-                    const u64 e = sh.list[tid];
-                    const uint32_t k = (uint32_t)(e >> 32), j = (uint32_t)e;
-                    int ro = 0, ri = 0;
-#pragma unroll 4
-                    for (int q = 0; q < m; ++q) {
-                        const u64 x = sh.list[q];
-                        const uint32_t xk = (uint32_t)(x >> 32), xj = (uint32_t)x;
-                        ri += xj < j;
-                        ro += xk > k || (xk == k && xj < j);
+                const int m = all_of;
+                if (m <= RANKED) {
+                    u64 e = 0;
+                    if (tid < m) {
+                        e = sh.list[tid];
+                        const uint32_t k = (uint32_t)(e >> 32), j = (uint32_t)e;
+                        int ro = 0, ri = 0;
+                        for (int q = 0; q < m; ++q) {
+                            const u64 x = sh.list[q];
+                            const uint32_t xk = (uint32_t)(x >> 32), xj = (uint32_t)x;
+                            ri += xj < j;
+                            ro += xk > k || (xk == k && xj < j);
+                        }
+                        sh.order[ro] = weigh(k);
+                        sh.place[ri] = ro | (weigh.real(k) < mp_units ? 0x80000000u : 0u);
+                        sh.index[ri] = j;
                     }
-                    by_order[ro] = weigh(k);
-                    place[ri] = ro | (weigh.real(k) < mp_units ? 0x80000000u : 0u);
-                    place[LOCAL + ri] = j;
-                }
-                __syncthreads();
-                u64 w = tid < m && (!use_k || (u64)tid < kk) ? by_order[tid] : 0ull;
-                u64 run = scan(w);
-                const u64 sum = block_sum(w);
-                if (use_k) W = sum;  // what top-k leaves
-                const double t = ceil((double)fmaxf(p, 0.0f) * (double)W);
-                const u64 want = p < 1.0f ? (t < 1.0 ? 1ull : (u64)t) : ~0ull;
-                if (tid == 0) sh.found = p < 1.0f && sum < want ? -2 : -1;  // -2: the cut lies behind the list
-                if (tid < m) by_order[tid] = run < want ? w : 0ull;  // stays where what precedes it has not reached the whole
-                __syncthreads();
-                if (sh.found != -2) {
-                    const uint32_t q = tid < m ? place[tid] : 0x80000000u;
-                    w = q & 0x80000000u ? 0ull : by_order[q];
-                    run = scan(w);
-                    const u64 K = block_sum(w);
-                    const double uu = u_in > 0.0f ? (double)u_in : 0.0;
-                    u64 tt = uu >= 1.0 ? K - 1 : (u64)(uu * (double)K);
-                    if (tt > K - 1) tt = K - 1;
-                    if (run <= tt && tt < run + w) sh.found = (int)place[LOCAL + tid];
-                }
-                __syncthreads();
-            }
-            int token = -1;
-            gather(rank == 0 ? (u64)(uint32_t)sh.found : 0ull, [&](uint32_t r, u64 x) { token = r == 0 ? (int)(uint32_t)x : token; });
-            if (token >= 0) return done(token);
-        } else {
-            if (use_k) {
-                auto one = [](uint32_t k, uint32_t) { return k ? 1ull : 0ull; };
-                if (n_k <= LIST) {
-                    to_list(bk, bk);
-                    cut_list(k_left, one, [](uint32_t) { return 1ull; });
+                    __syncthreads();
+                    u64 v = tid < m && (!use_k || (u64)tid < kk) ? sh.order[tid] : 0ull;
+                    u64 run = scan(v);
+                    if (use_k) W = block_sum(v);  // what top-k leaves
+                    const u64 want = has_p ? part_of(W) : ~0ull;
+                    if (tid < m) sh.order[tid] = run < want ? v : 0ull;  // stays where what precedes it has not reached the part
+                    __syncthreads();
+                    const uint32_t q = tid < m ? sh.place[tid] : 0x80000000u;
+                    v = q & 0x80000000u ? 0ull : sh.order[q];
+                    run = scan(v);
+                    const u64 t = pick(block_sum(v));
+                    if (run <= t && t < run + v) a.out[row] = (int)sh.index[tid];
                 } else {
-                    cut_row(kk, one, [](uint32_t) { return 1ull; });
+                    if (use_k) {
+                        list_load(false);
+                        list_cut(kk, false);
+                    }
+                    list_load(true);
+                    if (has_p) {
+                        if (use_k) W = list_sum([&](uint32_t k, uint32_t j, u64 v) { return stays(k, j) ? v : 0ull; });
+                        list_cut(part_of(W), true);
+                    }
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (!stays(lk[e], lj[e]) || weigh.real(lk[e]) < mp_units) lw[e] = 0;
+                    const u64 t = pick(list_sum([](uint32_t, uint32_t, u64 v) { return v; }));
+                    uint32_t l = 0, at = a.vocab;  // the sum over indexes below l is at most t, that below `at` exceeds it
+                    while (at - l > 1) {
+                        const uint32_t mid = (l + at) / 2;
+                        if (list_sum([&](uint32_t, uint32_t j, u64 v) { return j < mid ? v : 0ull; }) > t) at = mid;
+                        else l = mid;
+                    }
+                    if (tid == 0) a.out[row] = (int)at - 1;
                 }
             }
-            if (p < 1.0f) {
-                auto f = [&](uint32_t k, uint32_t j) { return stays(k, j) ? weigh(k) : 0ull; };
-                u64 above = 0;
-                if (use_k) W = over(f);
-                const double t = ceil((double)fmaxf(p, 0.0f) * (double)W);
-                const u64 want = t < 1.0 ? 1ull : (u64)t;
-                bool in_list = !use_k && n_p <= LIST;
-                if (in_list) {
-                    to_list(p0, p1);
-                    above = over([&](uint32_t k, uint32_t j) { return k && bin_of(k) < p0 ? f(k, j) : 0ull; });
-                    const u64 inside = over([&](uint32_t k, uint32_t j) {
-                        if (!k) return 0ull;
-                        const int b = bin_of(k);
-                        return b >= p0 && b <= p1 ? f(k, j) : 0ull;
-                    });
-                    in_list = above < want && want <= above + inside;
-                }
-                if (in_list) cut_list(want - above, f, [&](uint32_t k) { return weigh(k); });
-                else cut_row(want, f, [&](uint32_t k) { return weigh(k); });
-            }
-            goto draw;
+            return;  // (the others' shared memory is not read any more)
         }
-        // the candidates did not hold top-p's cut: over the row
-        {
-            if (use_k) cut_row(kk, [](uint32_t k, uint32_t) { return k ? 1ull : 0ull; }, [](uint32_t) { return 1ull; });
+        if (use_k) {
+            if (n_k <= LIST) {
+                to_list(bk, bk);
+                cut_list(kk - before_k, false);
+            } else {
+                cut_row(kk, [](uint32_t k, uint32_t) { return k ? 1ull : 0ull; }, [](uint32_t) { return 1ull; });
+            }
+        }
+        if (has_p) {
             auto f = [&](uint32_t k, uint32_t j) { return stays(k, j) ? weigh(k) : 0ull; };
-            if (use_k) W = over(f);
-            const double t = ceil((double)fmaxf(p, 0.0f) * (double)W);
-            cut_row(t < 1.0 ? 1ull : (u64)t, f, [&](uint32_t k) { return weigh(k); });
+            if (use_k) {
+                W = over(f);
+                find_weight(part_of(W));
+            }
+            const u64 want = part_of(W);
+            if (n_p <= LIST) {
+                to_list(bp, bp);
+                cut_list(want - above, true);
+            } else {
+                cut_row(want, f, [&](uint32_t k) { return weigh(k); });
+            }
         }
     }
-draw:
     // the draw: each warp sums a run of consecutive entries
-    auto kept = [&](int i) -> u64 {
-        const uint32_t k = i < n ? keys[i] : 0u;
-        if (!k || !stays(k, (uint32_t)(base + i))) return 0;
+    auto kept = [&](uint32_t k) -> u64 {  // of a key that stays
         const double w = weigh.real(k);
-        return w < mp_units ? 0ull : Weigh::whole(w);
+        return k == 0 || w < mp_units ? 0ull : Weigh::whole(w);
     };
     const int run_len = ((a.slice + WARPS - 1) / WARPS + 31) / 32 * 32, i0 = warp * run_len, i1 = min(i0 + run_len, n);
     u64 mine = 0;
-    for (int i = i0 + lane; i < i1; i += 32) mine += kept(i);
+    if (ck == 1) {  // no cut
+        for (int i = i0 + lane; i < i1; i += 32) mine += kept(keys[i]);
+    } else {  // what stays is queued, so that weights are computed for 32 of them at a time
+        uint32_t *queue = sh.queue[warp];
+        int q = 0;
+        for (int i = i0; i < i1; i += 32) {
+            const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
+            const bool in = k && stays(k, (uint32_t)(base + i + lane));
+            const uint32_t who = __ballot_sync(~0u, in);
+            if (in) queue[q + __popc(who & ((1u << lane) - 1))] = k;
+            q += __popc(who);
+            __syncwarp();
+            if (q >= 32) {
+                mine += kept(queue[lane]);
+                const uint32_t rest = queue[32 + lane];
+                __syncwarp();
+                queue[lane] = rest;
+                q -= 32;
+                __syncwarp();
+            }
+        }
+        if (lane < q) mine += kept(queue[lane]);
+    }
     mine = warp_sum(mine);
     __syncthreads();
     if (lane == 0) sh.warp[0][warp] = mine;
-    if (tid == 0) sh.found = -1;
     __syncthreads();
     u64 before = 0, all = 0;
     for (int k = 0; k < WARPS; ++k) {
@@ -535,13 +674,12 @@ draw:
         if (r < rank) front += x;
         K += x;
     });
-    const double uu = u_in > 0.0f ? (double)u_in : 0.0;
-    u64 t = uu >= 1.0 ? K - 1 : (u64)(uu * (double)K);
-    if (t > K - 1) t = K - 1;
+    const u64 t = pick(K);
     before += front;
     if (before <= t && t < before + mine) {  // this warp's run holds it
         for (int i = i0; i < i1; i += 32) {
-            u64 x = kept(i + lane < i1 ? i + lane : n);
+            const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
+            u64 x = k && stays(k, (uint32_t)(base + i + lane)) ? kept(k) : 0ull;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const u64 y = __shfl_up_sync(~0u, x, d);
