@@ -105,8 +105,8 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t a, uint32_t v) {
     return r;
 }
 
-struct Shared {
-    double tab[64];      // 2^(j / 64)
+struct alignas(16) Shared {
+    double tab[16];      // 2^(j / 16)
     u64 warp[2][WARPS];  // block sums
     u64 red[2][3];       // this CTA's part of what a cluster shares
     uint32_t n_list;
@@ -123,34 +123,58 @@ struct Shared {
     };
 };
 
-// The weight's arithmetic: 2^y by a table of 2^(j / 64) and the series of 2^r, |r| <= 1/128 (the first term left out is
-// below 2^-54).
+static_assert(sizeof(Shared) % 16 == 0, "the keys behind it are read 16 bytes at a time");
+
+// The weight's arithmetic: 2^y by a table of 2^(j / 16), whose entries no two banks share, and the series of 2^r,
+// |r| <= 1/32 (the first term left out is below 2^-51, a hundredth of a unit). No branches: several run at a time.
 struct Weigh {
     double c, xmax;  // log2(e) / T
     uint32_t kmax;
     bool inf;
     const double *tab;
     __device__ __forceinline__ double real(uint32_t k) const {  // in units
-        if (k == kmax) return 17592186044416.0;
         const double y = ((double)value_of(k) - xmax) * c;
-        if (inf || !(y > -46.0)) return 0.0;
-        const double t = fma(y, 64.0, 6755399441055744.0);  // rounds to an integer in the low bits
+        const double t = fma(y, 16.0, 6755399441055744.0);  // rounds to an integer in the low bits
         const int n = __double2loint(t);
-        const double r = fma(t - 6755399441055744.0, -0.015625, y);
-        double p = 0.00133335581464284434;  // ln(2)^n / n!
-        p = fma(p, r, 0.00961812910762847716);
-        p = fma(p, r, 0.0555041086648215800);
-        p = fma(p, r, 0.240226506959100712);
-        p = fma(p, r, 0.693147180559945309);
+        const double r = fma(t - 6755399441055744.0, -0.0625, y);
+        double p = 0.000154035303933816061;  // ln(2)^n / n!
+        p = fma(p, r, 0.00133335581464284411);
+        p = fma(p, r, 0.00961812910762847688);
+        p = fma(p, r, 0.0555041086648215762);
+        p = fma(p, r, 0.240226506959100694);
+        p = fma(p, r, 0.693147180559945286);
         p = fma(p, r, 1.0);
-        p *= tab[n & 63];
-        return __hiloint2double(__double2hiint(p) + (((n >> 6) + 44) << 20), __double2loint(p));
+        p *= tab[n & 15];
+        p = __hiloint2double(__double2hiint(p) + (((n >> 4) + 44) << 20), __double2loint(p));
+        return k == kmax ? 17592186044416.0 : !inf && y > -46.0 ? p : 0.0;  // (of key 0, NaN: 0)
     }
     static __device__ __forceinline__ u64 whole(double w) {  // w below 2^51, to the nearest
         return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ u64 operator()(uint32_t k) const { return k ? whole(real(k)) : 0ull; }
+    __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
 };
+
+// Values of 16 bits leave the low bits of their keys alike: a bisection over keys need not look at them.
+template <typename T>
+struct Spare;
+template <>
+struct Spare<float> {
+    static constexpr int bits = 0;
+};
+template <>
+struct Spare<__half> {
+    static constexpr int bits = 13;
+};
+template <>
+struct Spare<__nv_bfloat16> {
+    static constexpr int bits = 16;
+};
+template <typename T>
+__device__ __forceinline__ uint32_t key_at(uint32_t q) {  // the key whose upper bits are q
+    constexpr int b = Spare<T>::bits;
+    const uint32_t k = q << b;
+    return k & 0x80000000u ? k : k | ((1u << b) - 1u);
+}
 
 // sum over the warp, below 2^63: three parts of 26 bits whose sums stay in 32
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -167,7 +191,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     const uint32_t rank = cluster_rank(), C = cluster_size();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = (int)rank * a.slice, n = max(0, min(a.slice, a.vocab - base));
-    if (tid < 64) sh.tab[tid] = exp2(tid / 64.0);
+    if (tid < 16) sh.tab[tid] = exp2(tid / 16.0);
     pdl_wait();
     const float T_ = a.temp ? a.temp[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const float mp = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
@@ -183,6 +207,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         __syncthreads();
         v = lane < WARPS ? w[lane] : 0;
         return warp_sum(v);
+    };
+    auto block_count = [&](uint32_t v) {
+        v = __reduce_add_sync(~0u, v);
+        u64 *w = sh.warp[flip & 1];
+        ++flip;
+        if (lane == 0) w[warp] = v;
+        __syncthreads();
+        return __reduce_add_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : 0u);
     };
     int turn = 0;
     // every CTA's values (v, x, y: the same in all its threads, or those of the thread that names them by `mine`): f(rank, v, x, y)
@@ -251,6 +283,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         }
         if (tail + tid < n) put(tail + tid, to_f(x[tail + tid]));
     }
+    if (tid < 4 && n + tid < (n + 3) / 4 * 4) keys[n + tid] = 0;  // read four at a time
     top = __reduce_max_sync(~0u, top);
     if (lane == 0) sh.warp[0][warp] = top;
     __syncthreads();
@@ -297,11 +330,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     // Bisection over the row: the largest key whose sum over keys >= it reaches `want`, and the smallest count of its
     // first equals that does.
     auto cut_row = [&](u64 want, auto f, auto per_equal) {
+        constexpr int sp = Spare<T>::bits;
         uint32_t c = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        for (uint32_t bit = 0x80000000u >> sp; bit; bit >>= 1) {
             const uint32_t t = c | bit;
-            if (over([&](uint32_t k, uint32_t j) { return k >= t ? f(k, j) : 0ull; }) >= want) c = t;
+            if (over([&](uint32_t k, uint32_t j) { return k >> sp >= t ? f(k, j) : 0ull; }) >= want) c = t;
         }
+        c = key_at<T>(c);
         const u64 above = over([&](uint32_t k, uint32_t j) { return k > c ? f(k, j) : 0ull; });
         const u64 w = per_equal(c), m = (want - above + w - 1) / w;
         uint32_t lo = 0, hi = a.vocab;
@@ -333,6 +368,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         for (int e = 0; e < PER; ++e) s += f(lk[e], lj[e], lw[e]);
         return block_sum(s);
     };
+    auto list_count = [&](auto f) {
+        uint32_t s = 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) s += f(lk[e], lj[e]) ? 1u : 0u;
+        return block_count(s);
+    };
     // the cut of the entries that stay at the first place where the sum of lw reaches `want`
     auto list_cut = [&](u64 want, bool weights) {
         uint32_t x = 0, y = ~0u;
@@ -350,10 +391,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         __syncthreads();
         uint32_t hi = __reduce_max_sync(~0u, lane < WARPS ? (uint32_t)(w[lane] >> 32) : 0u);
         uint32_t lo = __reduce_min_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : ~0u);
+        constexpr int sp = Spare<T>::bits;
+        lo >>= sp;
+        hi >>= sp;
         u64 above = 0;
         while (lo < hi) {  // the sum over keys >= lo reaches want, that over keys > hi, `above`, does not
             const uint32_t mid = lo + (hi - lo + 1) / 2;
-            const u64 s = list_sum([&](uint32_t k, uint32_t j, u64 v) { return k >= mid && stays(k, j) ? v : 0ull; });
+            const u64 s = list_sum([&](uint32_t k, uint32_t j, u64 v) { return k >> sp >= mid && stays(k, j) ? v : 0ull; });
             if (s >= want) {
                 lo = mid;
             } else {
@@ -361,16 +405,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
                 above = s;
             }
         }
-        const uint32_t c = lo;
+        const uint32_t c = key_at<T>(lo);
         const u64 each = weights ? weigh(c) : 1ull, take = (want - above + each - 1) / each;
-        const u64 have = list_sum([&](uint32_t k, uint32_t j, u64) { return k == c && stays(k, j) ? 1ull : 0ull; });
+        const u64 have = list_count([&](uint32_t k, uint32_t j) { return k == c && stays(k, j); });
         uint32_t at = ck == c ? ci : ~0u;  // all of the equals that stay
         if (take < have) {
             uint32_t l = 0;
             at = a.vocab;
             while (at - l > 1) {
                 const uint32_t mid = (l + at) / 2;
-                if (list_sum([&](uint32_t k, uint32_t j, u64) { return k == c && j < mid && stays(k, j) ? 1ull : 0ull; }) >= take) at = mid;
+                if (list_count([&](uint32_t k, uint32_t j) { return k == c && j < mid && stays(k, j); }) >= take) at = mid;
                 else l = mid;
             }
         }
@@ -391,11 +435,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     // live entries whose bin is in [b0, b1] and that stay, into the first CTA's list
     auto to_list = [&](int b0, int b1) {
         u64 in = 0;  // of this thread's entries
-        for (int i = tid, e = 0; i < n; i += THREADS, ++e) {
-            const uint32_t k = keys[i];
-            if (k == 0) continue;
-            const int b = bin_of(k);
-            if (b >= b0 && b <= b1 && stays(k, (uint32_t)(base + i))) in |= 1ull << e;
+        for (int i = tid * 4, e = 0; i < n; i += THREADS * 4, e += 4) {
+            const uint4 k4 = *reinterpret_cast<const uint4 *>(keys + i);
+            const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(k[j]);
+                if (k[j] && b >= b0 && b <= b1 && stays(k[j], (uint32_t)(base + i + j))) in |= 1ull << (e + j);
+            }
         }
         if (tid == 0) sh.n_list = 0;
         cluster_sync();  // (the histograms, which lie under the list, have been read)
@@ -412,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         const uint32_t dst = remote(sh.list, 0);
         for (; in; in &= in - 1, ++at)
             if (at < LIST) {
-                const int i = tid + (__ffsll((long long)in) - 1) * THREADS;
+                const int e = __ffsll((long long)in) - 1, i = (tid + e / 4 * THREADS) * 4 + e % 4;
                 remote_store(dst + at * 8, (u64)keys[i] << 32 | (uint32_t)(base + i));
             }
         __syncwarp();
@@ -433,17 +480,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     if (kk || has_p) {
         for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.low[i] = sh.high[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += THREADS) {
-            const uint32_t k = keys[i];
-            if (k == 0) continue;
-            const int b = bin_of(k);
-            atomicAdd(&sh.count[b], 1u);
-            if (has_p) {
-                const u64 w = weigh(k);
-                const uint32_t lo = (uint32_t)w;
-                uint32_t hi = (uint32_t)(w >> 32);
-                if (lo && atomicAdd(&sh.low[b], lo) > ~lo) ++hi;
-                if (hi) atomicAdd(&sh.high[b], hi);
+        for (int i = tid * 4; i < n; i += THREADS * 4) {
+            const uint4 k4 = *reinterpret_cast<const uint4 *>(keys + i);
+            const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+            int b[4];
+            u64 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                b[e] = bin_of(k[e]);
+                w[e] = has_p ? weigh(k[e]) : 0ull;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (k[e] == 0) continue;
+                atomicAdd(&sh.count[b[e]], 1u);
+                const uint32_t lo = (uint32_t)w[e];
+                uint32_t hi = (uint32_t)(w[e] >> 32);
+                if (lo && atomicAdd(&sh.low[b[e]], lo) > ~lo) ++hi;
+                if (hi) atomicAdd(&sh.high[b[e]], hi);
             }
         }
         __syncwarp();
