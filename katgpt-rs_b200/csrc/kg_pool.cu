@@ -25,6 +25,9 @@ namespace {
 // the requests (new tokens, new pages) place everything: page i of the step is
 // free[n_free - 1 - i] and belongs to the request whose page range holds i,
 // token t to the request whose token range holds t.
+// Bound by latency: one launch. A cluster of 1 or 8 CTAs; each computes the running
+// sums for itself (a few loads a thread), the checks meet at a cluster barrier
+// before anything is written, and the tokens and pages are shared out.
 struct PlanArgs {
     int page, n_pages, n_req, width, max_tokens;
     const int32_t *cached, *fresh;
@@ -45,37 +48,41 @@ __device__ __forceinline__ int range_of(const int32_t *cum, int n, int i) {
     }
     return lo;
 }
+__device__ __forceinline__ int pages_of(long long positions, int shift) { return (int)((positions + (1 << shift) - 1) >> shift); }
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs a) {
-    pdl_wait();
     extern __shared__ int32_t sm[];
-    int32_t *cu = sm, *pg = sm + a.n_req + 1;  // running sums of new tokens and new pages
+    int32_t *cu = sm, *pg = sm + a.n_req + 1, *old = pg + a.n_req + 1;  // running sums of new tokens and new pages; cached lengths
     __shared__ long long wt[32], wp[32], s_tot[2];
-    __shared__ int s_bad, s_free;
+    __shared__ int s_bad;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) {
-        s_bad = 0;
-        s_free = *a.n_free;
-    }
-    __syncthreads();
+    uint32_t rank, ctas;
+    asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %cluster_nctarank;" : "=r"(ctas));
+    const int shift = 31 - __clz(a.page), gid = (int)rank * PLAN_THREADS + tid, step = (int)ctas * PLAN_THREADS;
+    if (tid == 0) s_bad = 0;
+    pdl_wait();
+    const int nf = *a.n_free;
     const int per = (a.n_req + PLAN_THREADS - 1) / PLAN_THREADS;
     const int r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
     long long t = 0, p = 0;
-    bool bad = false;
+    bool bad = nf < 0 || nf > a.n_pages;
     for (int r = r0; r < r1; ++r) {
         const long long c = a.cached[r], n = a.fresh[r], end = c + n;
-        if (c < 0 || n < 0 || end > INT32_MAX || (end + a.page - 1) / a.page > a.width) {
+        if (c < 0 || n < 0 || end > INT32_MAX || pages_of(end, shift) > a.width) {
             bad = true;
             continue;
         }
-        if (n > 0 && c % a.page) {  // its last page takes new rows
-            const int e = a.table[(int64_t)r * a.width + c / a.page];
+        old[r] = (int)c;
+        if (n > 0 && c & (a.page - 1)) {  // its last page takes new rows
+            const int e = a.table[(int64_t)r * a.width + (c >> shift)];
             bad |= e < 0 || e >= a.n_pages;
         }
         t += n;
-        p += (end + a.page - 1) / a.page - (c + a.page - 1) / a.page;
+        p += pages_of(end, shift) - pages_of(c, shift);
     }
     long long it = t, ip = p;  // inclusive sums over the block's threads
+#pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const long long u = __shfl_up_sync(~0u, it, d), v = __shfl_up_sync(~0u, ip, d);
         if (lane >= d) {
@@ -87,75 +94,96 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs a) {
         wt[warp] = it;
         wp[warp] = ip;
     }
-    __syncthreads();
-    long long bt = 0, bp = 0;
-    for (int w = 0; w < warp; ++w) {
-        bt += wt[w];
-        bp += wp[w];
-    }
-    if (tid == PLAN_THREADS - 1) {
-        s_tot[0] = bt + it;
-        s_tot[1] = bp + ip;
-    }
+    __syncthreads();  // (s_bad is 0 by now)
     if (bad) s_bad = 1;
+    if (warp == 0) {
+        long long x = wt[lane], y = wp[lane];
+        const long long x0 = x, y0 = y;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long u = __shfl_up_sync(~0u, x, d), v = __shfl_up_sync(~0u, y, d);
+            if (lane >= d) {
+                x += u;
+                y += v;
+            }
+        }
+        if (lane == 31) {
+            s_tot[0] = x;
+            s_tot[1] = y;
+        }
+        wt[lane] = x - x0;
+        wp[lane] = y - y0;
+    }
     __syncthreads();
-    const int nf = s_free;
     const long long tokens = s_tot[0], pages = s_tot[1];
     int code = KG_OK;
-    if (s_bad || tokens > a.max_tokens || nf < 0 || nf > a.n_pages) code = KG_ERR_INVALID_ARG;
+    if (s_bad || tokens > a.max_tokens) code = KG_ERR_INVALID_ARG;
     else if (pages > nf) code = KG_ERR_OOM;
     if (code == KG_OK) {
-        bt += it - t;
-        bp += ip - p;
+        long long bt = wt[warp] + it - t, bp = wp[warp] + ip - p;
         for (int r = r0; r < r1; ++r) {
-            const int c = a.cached[r], n = a.fresh[r];
+            const int n = a.fresh[r];
+            const long long c = old[r];
             cu[r] = (int)bt;
             pg[r] = (int)bp;
             bt += n;
-            bp += (int)(((long long)c + n + a.page - 1) / a.page) - (int)(((long long)c + a.page - 1) / a.page);
+            bp += pages_of(c + n, shift) - pages_of(c, shift);
         }
         if (tid == 0) {
             cu[a.n_req] = (int)tokens;
             pg[a.n_req] = (int)pages;
         }
-        for (int i = tid; i < (int)pages; i += PLAN_THREADS) {
+        for (int i = gid; i < (int)pages; i += step) {
             const int e = a.free_pages[nf - 1 - i];
             if (e < 0 || e >= a.n_pages) s_bad = 1;
         }
     }
     __syncthreads();
-    if (s_bad) code = KG_ERR_INVALID_ARG;
-    if (tid == 0) {
+    if (ctas > 1) {  // every CTA has read the free count and checked its share; nothing has been written
+        asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;\n" ::: "memory");
+        int other = 0;
+        if (lane < (int)ctas) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_bad)), "r"(lane));
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(other) : "r"(at) : "memory");
+        }
+        if (__any_sync(~0u, other != 0)) code = KG_ERR_INVALID_ARG;
+        asm volatile("barrier.cluster.arrive.release;\n" ::: "memory");  // (waited for at the end: no CTA leaves before it has been read)
+    } else if (s_bad) {
+        code = KG_ERR_INVALID_ARG;
+    }
+    if (gid == 0) {
         *a.status = code;
         *a.n_free_out = code == KG_OK ? nf - (int)pages : nf;
     }
     if (code != KG_OK) {  // the step does nothing
-        for (int r = tid; r <= a.n_req; r += PLAN_THREADS) a.cu[r] = 0;
-        for (int r = tid; r < a.n_req; r += PLAN_THREADS) a.kv[r] = 0;
-        for (int i = tid; i < a.max_tokens; i += PLAN_THREADS) a.slots[i] = a.req[i] = a.pos[i] = -1;
-        return;
-    }
-    for (int r = tid; r <= a.n_req; r += PLAN_THREADS) a.cu[r] = cu[r];
-    for (int r = tid; r < a.n_req; r += PLAN_THREADS) a.kv[r] = a.cached[r] + a.fresh[r];
-    for (int i = tid; i < (int)pages; i += PLAN_THREADS) {
-        const int r = range_of(pg, a.n_req, i);
-        const int has = (int)(((long long)a.cached[r] + a.page - 1) / a.page);
-        a.table[(int64_t)r * a.width + has + i - pg[r]] = a.free_pages[nf - 1 - i];
-    }
-    for (int i = tid; i < a.max_tokens; i += PLAN_THREADS) {
-        int slot = -1, r = -1, x = -1;
-        if (i < (int)tokens) {
-            r = range_of(cu, a.n_req, i);
-            const int c = a.cached[r];
-            x = c + i - cu[r];
-            const int has = (int)(((long long)c + a.page - 1) / a.page), q = x / a.page;
-            const int e = q < has ? a.table[(int64_t)r * a.width + q] : a.free_pages[nf - 1 - (pg[r] + q - has)];
-            slot = e * a.page + x % a.page;
+        for (int r = gid; r <= a.n_req; r += step) a.cu[r] = 0;
+        for (int r = gid; r < a.n_req; r += step) a.kv[r] = 0;
+        for (int i = gid; i < a.max_tokens; i += step) a.slots[i] = a.req[i] = a.pos[i] = -1;
+    } else {
+        for (int r = gid; r <= a.n_req; r += step) a.cu[r] = cu[r];
+        for (int r = gid; r < a.n_req; r += step) a.kv[r] = old[r] + cu[r + 1] - cu[r];
+        for (int i = gid; i < (int)pages; i += step) {
+            const int r = range_of(pg, a.n_req, i);
+            a.table[(int64_t)r * a.width + pages_of(old[r], shift) + i - pg[r]] = a.free_pages[nf - 1 - i];
         }
-        a.slots[i] = slot;
-        a.req[i] = r;
-        a.pos[i] = x;
+#pragma unroll 4
+        for (int i = gid; i < a.max_tokens; i += step) {
+            int slot = -1, r = -1, x = -1;
+            if (i < (int)tokens) {
+                r = range_of(cu, a.n_req, i);
+                const int c = old[r];
+                x = c + i - cu[r];
+                const int has = pages_of(c, shift), q = x >> shift;
+                const int e = __ldg(q < has ? a.table + (int64_t)r * a.width + q : a.free_pages + (nf - 1 - (pg[r] + q - has)));
+                slot = (e << shift) + (x & (a.page - 1));
+            }
+            a.slots[i] = slot;
+            a.req[i] = r;
+            a.pos[i] = x;
+        }
     }
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -251,10 +279,11 @@ int kg_pool_plan_dev(kg_ctx *ctx, int32_t page_size, int32_t n_pages, int32_t n_
     if (dg.err != cudaSuccess) return cuda_fail(ctx, dg.err, "kg_pool_plan_dev");
     PlanArgs a{page_size, n_pages, n_req, table_width, max_tokens, cached_len, new_len, table, free_pages,
                n_free, n_free_out, cu_q, kv_len, slots, req_of, positions, status};
-    const size_t smem = (size_t)(2 * n_req + 2) * sizeof(int32_t);
-    cudaError_t e = smem > 48 * 1024 ? kg::dev::smem(plan_kernel, smem) : cudaSuccess;
+    const size_t smem = (size_t)(3 * n_req + 2) * sizeof(int32_t);
+    const int ctas = max_tokens > 2 * PLAN_THREADS || n_req > 2 * PLAN_THREADS ? 8 : 1;
+    cudaError_t e = smem > 40 * 1024 ? kg::dev::smem(plan_kernel, smem) : cudaSuccess;
     if (e == cudaSuccess)
-        e = kg::launch_pdl(plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), a);
+        e = kg::launch_pdl_cluster(plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), dim3(ctas), a);
     return e == cudaSuccess ? KG_OK : cuda_fail(ctx, e, "kg_pool_plan_dev");
 }
 
