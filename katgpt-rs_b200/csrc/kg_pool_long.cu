@@ -257,6 +257,16 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 if (n0 > 0) scores(0, it);
                 if (n1 > 0) scores(1, it);
                 release(it, n0 > 0 || n1 > 0);
+                // The item's last scores have been issued: the next item's rows of q may come once they are done, while
+                // this item's last values are still to do.
+                auto release_q = [&]() {
+                    if (elect()) {
+                        if (n0 > 0 || n1 > 0) tc::commit(qempty);
+                        else mbar_arrive(qempty);
+                    }
+                    __syncwarp();
+                };
+                if (w.n == 1) release_q();
                 for (int u = 0; ok && u < w.n; ++u, it += 2) {
                     const bool more = u + 1 < w.n;
                     if (!(ok = wait_slot(it + 1))) break;
@@ -269,12 +279,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     release(it + 1, u < n0 || u < n1);
                     if (u + 1 < n1) scores(1, it + 2);
                     if (more) release(it + 2, u + 1 < n0 || u + 1 < n1);
+                    if (u + 2 == w.n) release_q();
                 }
-                if (elect()) {
-                    if (n0 > 0 || n1 > 0) tc::commit(qempty);
-                    else mbar_arrive(qempty);
-                }
-                __syncwarp();
                 ++item;
             } while (ok && w.next(a));
         }
