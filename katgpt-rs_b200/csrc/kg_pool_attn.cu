@@ -30,15 +30,17 @@ using namespace as;
 // ---------------------------------------------------------------------------
 // Short requests (at most 64 rows: single tokens, draft paths) on mma.sync:
 // rows (token, query head of the group) x positions. Bound by the bytes of K and
-// V; a producer warp keeps a ring of 64-position stages filled by TMA, one box
-// per page, and four warps split a stage by rows (groups of 16) and by positions.
+// V; a producer warp keeps a ring of three 32 KB stages (64 positions of 128
+// dimensions, 128 of 64) filled by TMA, one box per page, and four warps split a
+// stage by rows (groups of 16) and by positions, 32 at a time where they have them.
 // Each keeps its own running maximum and sum, joined at the end of the item.
 constexpr int SHORT_THREADS = 160, SHORT_LEAST = 2;
 
 template <int D>
 struct ShortCfg {
-    static constexpr int OP_BYTES = kShortUnit * D * 2;  // K or V of a stage
-    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int UNIT = 64 * 128 / D;       // positions
+    static constexpr int OP_BYTES = UNIT * D * 2;  // K or V of a stage
+    static constexpr int STAGES = 3;
     static constexpr int SCRATCH = 4 * 16 * 36 * 4;
     static constexpr int SMEM = 1024 + STAGES * 2 * OP_BYTES + SCRATCH + 4 * 16 * 2 * 4 + 2 * STAGES * 8 + 16;
 };
@@ -105,14 +107,14 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     w.start(a, req, off, units);
 
     if (warp == 4) {  // producer: lane i loads box i of a unit
-        const int rows = min(a.page_size, kShortUnit), pages = kShortUnit / rows, boxes = pages * 2;
+        const int rows = min(a.page_size, kBoxRows), pages = C::UNIT / rows, boxes = pages * 2;
         const int piece = lane % pages, which = lane / pages;
         const CUtensorMap *tm = which ? &maps.v : &maps.k;
         const int dst = which * C::OP_BYTES + piece * rows * D * 2;
         int it = 0;
         do {
             for (int u = 0; u < w.n; ++u, ++it) {
-                const int s = it % C::STAGES, pos = (w.p.unit + u) * kShortUnit + piece * rows;
+                const int s = it % C::STAGES, pos = (w.p.unit + u) * C::UNIT + piece * rows;
                 int place = maps.outside;
                 if (lane < boxes && pos < w.kv) {
                     const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
@@ -167,11 +169,13 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
             const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, a.err);
             uint8_t *st = sm + s * 2 * C::OP_BYTES;
             bool wrote = false;
-            for (int b = 0; ok && b < wm; ++b) {
-                const int p0 = (pg * wm + b) * 16, pos0 = (w.p.unit + u) * kShortUnit + p0;
-                if (pos0 >= w.kv) break;
-                if (pos0 + 16 > w.kv) {  // rows behind the last position: whatever the page holds must not reach the sums
-                    for (int i = lane; i < 16 * (D / 8); i += 32) {
+            const int chunk = C::UNIT / 4 * wm, p_end = (pg + 1) * chunk, unit0 = (w.p.unit + u) * C::UNIT;
+            // positions p0 .. p0 + 16 NB of the stage
+            auto step = [&](auto nb, int p0) {
+                constexpr int NB = decltype(nb)::value;
+                const int pos0 = unit0 + p0;
+                if (pos0 + 16 * NB > w.kv) {  // rows behind the last position: whatever the page holds must not reach the sums
+                    for (int i = lane; i < 16 * NB * (D / 8); i += 32) {
                         const int r = i / (D / 8), ch = i % (D / 8);
                         if (pos0 + r >= w.kv)
                             *reinterpret_cast<uint4 *>(st + C::OP_BYTES + kv_offset<D>(p0 + r, ch)) = make_uint4(0, 0, 0, 0);
@@ -179,29 +183,28 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                     wrote = true;
                     __syncwarp();
                 }
-                float sc[2][4] = {};
-                {
-                    const int r = p0 + (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
-                    const uint32_t base = sa(st) + kv_offset<D>(r, 0);
+                float sc[2 * NB][4] = {};
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const int ch = k * 2 + cb;
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int r = p0 + b * 16 + (lane & 7) + ((lane >> 4) << 3), ch = k * 2 + ((lane >> 3) & 1);
                         uint32_t kf[4];
-                        ldsm4(base + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), kf);
-                        mma16816<T>(sc[0], qf[k], kf[0], kf[1]);
-                        mma16816<T>(sc[1], qf[k], kf[2], kf[3]);
+                        ldsm4(sa(st) + kv_offset<D>(r, 0) + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), kf);
+                        mma16816<T>(sc[2 * b], qf[k], kf[0], kf[1]);
+                        mma16816<T>(sc[2 * b + 1], qf[k], kf[2], kf[3]);
                     }
-                }
-                uint32_t pf[4];
+                uint32_t pf[NB][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float x[4];
+                    float x[4 * NB], mx = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2 * NB; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                        for (int e = 0; e < 2; ++e) {
                             x[n * 2 + e] = pos0 + n * 8 + tig * 2 + e < lim[i] ? sc[n][i * 2 + e] * a.scale : -INFINITY;
-                    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                            mx = fmaxf(mx, x[n * 2 + e]);
+                        }
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
                     const float mn = fmaxf(m[i], mx);
@@ -216,23 +219,35 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                         m[i] = mn;
                     }
                     const float base = mn == -INFINITY ? 0.0f : mn;
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e] - base);
-                    l[i] += (x[0] + x[1]) + (x[2] + x[3]);
-                    pf[i] = Cvt<T>::pack(x[0], x[1]);
-                    pf[i + 2] = Cvt<T>::pack(x[2], x[3]);
+                    for (int e = 0; e < 4 * NB; ++e) {
+                        x[e] = exp2_approx(x[e] - base);
+                        sum += x[e];
+                    }
+                    l[i] += sum;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        pf[b][i] = Cvt<T>::pack(x[4 * b], x[4 * b + 1]);
+                        pf[b][i + 2] = Cvt<T>::pack(x[4 * b + 2], x[4 * b + 3]);
+                    }
                 }
-                {
-                    const int r = p0 + (lane & 7) + (((lane >> 3) & 1) << 3), cb = lane >> 4;
-                    const uint32_t base = sa(st) + C::OP_BYTES + kv_offset<D>(r, 0);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        const int ch = k * 2 + cb;
+                        const int r = p0 + b * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), ch = k * 2 + (lane >> 4);
                         uint32_t vf[4];
-                        ldsm4t(base + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), vf);
-                        mma16816<T>(o[2 * k], pf, vf[0], vf[1]);
-                        mma16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+                        ldsm4t(sa(st) + C::OP_BYTES + kv_offset<D>(r, 0) + (ch >> 3) * 1024 + (((ch & 7) ^ (r & 7)) << 4), vf);
+                        mma16816<T>(o[2 * k], pf[b], vf[0], vf[1]);
+                        mma16816<T>(o[2 * k + 1], pf[b], vf[2], vf[3]);
                     }
+            };
+            if (ok) {
+                if (D == 128 && chunk == 16) {
+                    if (unit0 + pg * 16 < w.kv) step(std::integral_constant<int, 1>(), pg * 16);
+                } else {
+                    for (int p0 = pg * chunk; p0 < p_end && unit0 + p0 < w.kv; p0 += 32) step(std::integral_constant<int, 2>(), p0);
                 }
             }
             if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the stage again
@@ -409,7 +424,7 @@ bool pool_map(PoolMap &m, const kg_pool &p) {
     m.outside = (p.n_pages - 1) * m.page_step + (p.n_kv_head - 1) * m.head_step + 1;
     const cuuint64_t dims[5] = {64, 8, (cuuint64_t)p.head_dim / 64, (cuuint64_t)p.page_size / 8, (cuuint64_t)m.outside};
     const cuuint64_t strides[4] = {(cuuint64_t)rs * 2, 128, (cuuint64_t)rs * 16, (cuuint64_t)unit * 2};
-    const cuuint32_t box[5] = {64, 8, (cuuint32_t)p.head_dim / 64, (cuuint32_t)std::min(p.page_size, kShortUnit) / 8, 1};
+    const cuuint32_t box[5] = {64, 8, (cuuint32_t)p.head_dim / 64, (cuuint32_t)std::min(p.page_size, kBoxRows) / 8, 1};
     const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     for (int i = 0; i < 2; ++i)
         if (fn(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, i ? p.v : p.k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -518,7 +533,7 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
     DeviceGuard dg(ctx->device);
     if (dg.err != cudaSuccess) return cuda_fail(ctx, dg.err, "kg_pool_attend_dev");
     AttendArgs a;
-    a.s = Shape{n_head / pool->n_kv_head, pool->n_kv_head, 2 * (128 / (n_head / pool->n_kv_head)), causal != 0};
+    a.s = Shape{n_head / pool->n_kv_head, pool->n_kv_head, 2 * (128 / (n_head / pool->n_kv_head)), causal != 0, 64 * 128 / pool->head_dim};
     a.n_req = n_req;
     a.total_q = total_q;
     a.width = table_width;

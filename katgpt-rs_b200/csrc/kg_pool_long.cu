@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     };
 
     if (warp == 0) {  // loads
-        const int rows = min(a.page_size, kShortUnit), pages = kLongUnit / rows;  // a box each
+        const int rows = min(a.page_size, kBoxRows), pages = kLongUnit / rows;  // a box each
         int it = 0, item = 0;
         bool ok = true;
         do {

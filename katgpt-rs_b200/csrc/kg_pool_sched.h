@@ -2,7 +2,7 @@
 // arithmetic, used by the kernels and, compiled as C++, by a CPU test.
 //
 // A request whose rows (new tokens x query heads per K/V head) fit kShortRows
-// is "short": one item per K/V head, units of kShortUnit positions. The others
+// is "short": one item per K/V head, units of `unit` positions. The others
 // are "long": one item per (K/V head, tile of tokens), units of kLongUnit
 // positions up to the tile's last attended one. An item always has a unit, so
 // that rows which attend nothing get their zeros. The units of all items in
@@ -20,7 +20,7 @@
 namespace kg {
 namespace serve {
 
-constexpr int kShortRows = 64, kShortUnit = 64, kLongUnit = 128;
+constexpr int kShortRows = 64, kLongUnit = 128;
 constexpr int kMaxKv = 2147483647 - 256;  // a unit that begins before the last position ends inside 31 bits
 
 struct Shape {
@@ -28,6 +28,7 @@ struct Shape {
     int n_kv;       // K/V heads
     int tile;       // tokens of a long item
     int causal;
+    int unit;       // positions of a short item's unit
 };
 
 KG_HD bool lengths_ok(int q0, int q1, int kv, int total_q, int64_t room) {
@@ -38,7 +39,7 @@ KG_HD bool is_short(const Shape &s, int q) { return (int64_t)q * s.group <= kSho
 // units of one head's item of a short request (0: none)
 KG_HD int short_units(const Shape &s, int q, int kv) {
     if (q == 0 || !is_short(s, q)) return 0;
-    return kv > 0 ? (kv - 1) / kShortUnit + 1 : 1;
+    return kv > 0 ? (kv - 1) / s.unit + 1 : 1;
 }
 KG_HD int long_tiles(const Shape &s, int q) { return q == 0 || is_short(s, q) ? 0 : (q - 1) / s.tile + 1; }
 // positions that token t's row attends: [0, limit)

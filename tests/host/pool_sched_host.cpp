@@ -31,6 +31,7 @@ int main() {
         s.n_kv = 1 + rnd(4);
         s.tile = 2 * (128 / s.group);
         s.causal = rnd(2);
+        s.unit = rnd(2) ? 64 : 128;
         const int n_req = 1 + rnd(12);
         std::vector<int> q(n_req), kv(n_req);
         for (int r = 0; r < n_req; ++r) {
@@ -57,7 +58,7 @@ int main() {
                     for (int t = 0; t < tiles; ++t) {
                         const int units = is_long ? long_units(s, q[r], kv[r], t) : short_units(s, q[r], kv[r]);
                         const int last = is_long ? (t + 1) * s.tile < q[r] ? (t + 1) * s.tile - 1 : q[r] - 1 : q[r] - 1;
-                        const int lim = row_limit(s, q[r], kv[r], last), u = is_long ? kLongUnit : kShortUnit;
+                        const int lim = row_limit(s, q[r], kv[r], last), u = is_long ? kLongUnit : s.unit;
                         CHECK(units >= 1 && (long long)units * u >= lim && (units == 1 || (units - 1) * u < (is_long ? lim : kv[r])));
                         for (int i = 0; i < units; ++i, ++off) {
                             const Place p = place_of(s, is_long, q[r], kv[r], off);
@@ -75,7 +76,7 @@ int main() {
         }
     }
     // rows before position 0, lengths at their ends
-    Shape s{4, 2, 64, 1};
+    Shape s{4, 2, 64, 1, 64};
     CHECK(row_limit(s, 5, 2, 0) == 0 && row_limit(s, 5, 2, 4) == 2 && row_limit(s, 5, 2, 3) == 1);
     CHECK(row_limit(s, 1, 2147483647, 0) == 2147483647 && short_units(s, 1, 2147483647) == 33554432);
     CHECK(part_begin(1ll << 50, 511, 512) == (1ll << 50) / 512 * 511);
