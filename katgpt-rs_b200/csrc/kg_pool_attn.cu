@@ -317,12 +317,14 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     if (after_long) pdl_wait();
 }
 
-// Joins the parts of the items that were cut, of both kernels: block x looks after
-// the item that begins in part x and ends beyond it, eight rows a block in turn.
+// Joins the parts of the items that were cut, of both kernels: two blocks (eight for
+// the long requests' parts) look after the item that begins in a part and ends beyond
+// it, eight rows at a time. (A block for every eight rows there could be, 14 thousand
+// mostly empty ones, took 15 us.)
 // Few parts: a warp a row; many (a lone long sequence): the block's warps share a
 // row's parts. Part sums are added in a fixed order, so results do not depend on
 // timing.
-constexpr int JOIN_ROWS = 8, JOIN_FEW = 16;
+constexpr int JOIN_ROWS = 8, JOIN_FEW = 16, JOIN_SHORT = 2, JOIN_LONG = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, int short_parts, const AttendArgs lo) {
@@ -330,16 +332,17 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, i
     __shared__ int s_last;
     __shared__ float4 sums[8][32];
     __shared__ float part_l[8];
-    const bool is_long = (int)blockIdx.x >= short_parts;
+    const bool is_long = (int)blockIdx.x >= short_parts * JOIN_SHORT;
     const AttendArgs &a = is_long ? lo : sh;
-    const int c = is_long ? blockIdx.x - short_parts : blockIdx.x, parts = is_long ? gridDim.x - short_parts : short_parts;
+    const int per = is_long ? JOIN_LONG : JOIN_SHORT, x = is_long ? blockIdx.x - short_parts * JOIN_SHORT : blockIdx.x;
+    const int c = x / per, parts = is_long ? (gridDim.x - short_parts * JOIN_SHORT) / JOIN_LONG : short_parts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int4 me = a.meta[2 * c + 1];
     if (me.x == 0) return;
     int q0, q, kv;
     req_len(a, me.y, q0, q, kv);
     const int group = a.s.group, tq = a.s.tile / 2, rows = is_long ? 256 : q * group;
-    if ((int)blockIdx.y * JOIN_ROWS >= rows) return;
+    if (x % per * JOIN_ROWS >= rows) return;
     if (threadIdx.x == 0) {
         int e = c + 1;
         while (e < parts - 1 && a.meta[2 * e].x == 1) ++e;
@@ -349,8 +352,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, i
     const int n = s_last - c + 1;
     auto slot = [&](int i) { return a.part + (i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.slot_floats; };
     constexpr int PER = D / 32;  // dims of a lane
-    auto each = [&](int r) {     // row r of this block: token, or -1
-        const int row = blockIdx.y * JOIN_ROWS + r, i = is_long ? row & 127 : row;
+    auto each = [&](int row) {   // its token, or -1
+        const int i = is_long ? row & 127 : row;
         const int tok = is_long ? (me.w * 2 + (row >> 7)) * tq + i / group : i / group;
         return row >= rows || (is_long && i >= tq * group) || tok >= q ? -1 : tok;
     };
@@ -377,37 +380,39 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, i
 #pragma unroll
         for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t *>(dst)[e / 2] = Cvt<T>::pack(o[e] * inv, o[e + 1] * inv);
     };
-    if (n <= JOIN_FEW) {
-        const int tok = each(warp), row = blockIdx.y * JOIN_ROWS + warp;
-        if (tok < 0) return;
-        float o[PER] = {}, l = 0.0f;
-        sum_of(row, 0, 1, o, l);
-        write(row, tok, o, l);
-        return;
-    }
-    for (int r = 0; r < JOIN_ROWS; ++r) {
-        const int tok = each(r), row = blockIdx.y * JOIN_ROWS + r;
-        if (tok < 0) continue;
-        float o[PER] = {}, l = 0.0f;
-        sum_of(row, warp, 8, o, l);
-        sums[warp][lane] = make_float4(o[0], o[1], PER > 2 ? o[PER - 2] : 0.0f, PER > 2 ? o[PER - 1] : 0.0f);
-        if (lane == 0) part_l[warp] = l;
-        __syncthreads();
-        if (warp == 0) {
-            float t[PER] = {}, total = 0.0f;
-            for (int k = 0; k < 8; ++k) {
-                const float4 x = sums[k][lane];
-                t[0] += x.x;
-                t[1] += x.y;
-                if (PER > 2) {
-                    t[PER - 2] += x.z;
-                    t[PER - 1] += x.w;
-                }
-                total += part_l[k];
-            }
-            write(row, tok, t, total);
+    for (int row0 = x % per * JOIN_ROWS; row0 < rows; row0 += per * JOIN_ROWS) {
+        if (n <= JOIN_FEW) {
+            const int row = row0 + warp, tok = each(row);
+            if (tok < 0) continue;
+            float o[PER] = {}, l = 0.0f;
+            sum_of(row, 0, 1, o, l);
+            write(row, tok, o, l);
+            continue;
         }
-        __syncthreads();
+        for (int row = row0; row < row0 + JOIN_ROWS; ++row) {
+            const int tok = each(row);
+            if (tok < 0) continue;
+            float o[PER] = {}, l = 0.0f;
+            sum_of(row, warp, 8, o, l);
+            sums[warp][lane] = make_float4(o[0], o[1], PER > 2 ? o[PER - 2] : 0.0f, PER > 2 ? o[PER - 1] : 0.0f);
+            if (lane == 0) part_l[warp] = l;
+            __syncthreads();
+            if (warp == 0) {
+                float t[PER] = {}, total = 0.0f;
+                for (int k = 0; k < 8; ++k) {
+                    const float4 v = sums[k][lane];
+                    t[0] += v.x;
+                    t[1] += v.y;
+                    if (PER > 2) {
+                        t[PER - 2] += v.z;
+                        t[PER - 1] += v.w;
+                    }
+                    total += part_l[k];
+                }
+                write(row, tok, t, total);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -479,8 +484,7 @@ cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *worksp
     a.rows = sp.rows;
     e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a, (int)sp.may_long);
     if (e != cudaSuccess) return e;
-    const int rows = sp.may_long ? 256 : a.rows;
-    return launch_pdl(attend_join_kernel<T, D>, dim3(parts + long_parts, (rows + JOIN_ROWS - 1) / JOIN_ROWS), dim3(256), 0, s, a, parts, b);
+    return launch_pdl(attend_join_kernel<T, D>, dim3(parts * JOIN_SHORT + long_parts * JOIN_LONG), dim3(256), 0, s, a, parts, b);
 }
 
 int check(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q) {
