@@ -29,6 +29,7 @@ struct Tables {
     std::mutex mu;
     std::map<std::pair<int, const void *>, size_t> smem;           // (device, kernel) -> limit set
     std::map<std::tuple<int, const void *, int, size_t>, int> occ;  // (device, kernel, threads, smem) -> CTAs/SM
+    std::map<std::pair<int, const void *>, bool> carve;              // (device, kernel) -> carve-out set
     std::map<int, int> sms;                                         // device -> SM count
 };
 inline Tables &tables() {
@@ -50,6 +51,21 @@ inline cudaError_t smem_raw(const void *fn, size_t bytes) {
 template <typename... A>
 inline cudaError_t smem(void (*fn)(A...), size_t bytes) {
     return smem_raw(reinterpret_cast<const void *>(fn), bytes);
+}
+
+// `fn` runs with the SM's whole shared memory carved out, as its neighbours in a chain do: a kernel that wants another
+// division waits for the SM to empty first.
+template <typename... A>
+inline cudaError_t whole_smem(void (*fn)(A...)) {
+    const void *f = reinterpret_cast<const void *>(fn);
+    const int d = current();
+    Tables &t = tables();
+    std::lock_guard<std::mutex> lk(t.mu);
+    bool &done = t.carve[{d, f}];
+    if (done) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    done = e == cudaSuccess;
+    return e;
 }
 
 // SM count of the current device.

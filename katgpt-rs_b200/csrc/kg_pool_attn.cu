@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cstring>
 #include <type_traits>
@@ -464,9 +465,19 @@ cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *worksp
     std::memset(&maps, 0, sizeof(maps));
     if (!pool_map(maps, p)) return cudaErrorInvalidValue;
     using C = ShortCfg<D>;
-    cudaError_t e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
-    if (e != cudaSuccess) return e;
-    const int parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
+    // per device, once: attributes and the CTAs that the device holds
+    static std::atomic<int> held[64];
+    const int device = dev::current() & 63;
+    int parts = held[device].load(std::memory_order_acquire);
+    cudaError_t e = cudaSuccess;
+    if (parts == 0) {
+        e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
+        if (e == cudaSuccess) e = dev::whole_smem(attend_short_kernel<T, D>);
+        if (e == cudaSuccess) e = dev::whole_smem(attend_join_kernel<T, D>);
+        if (e != cudaSuccess) return e;
+        parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
+        held[device].store(parts, std::memory_order_release);
+    }
     AttendArgs b = a;
     int long_parts = 0;
     if (sp.may_long) {

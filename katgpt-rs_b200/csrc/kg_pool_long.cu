@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -457,8 +458,14 @@ cudaError_t launch(const PoolMap &kv, const AttendArgs &a, int parts, cudaStream
     maps.kv = kv;
     if (!q_map(&maps.q, a, D)) return cudaErrorInvalidValue;
     using C = LongCfg<D>;
-    cudaError_t e = dev::smem(attend_long_kernel<T, D>, C::SMEM);
-    if (e != cudaSuccess) return e;
+    static std::atomic<bool> set[64];  // attributes, per device
+    const int device = dev::current() & 63;
+    if (!set[device].load(std::memory_order_acquire)) {
+        cudaError_t e = dev::smem(attend_long_kernel<T, D>, C::SMEM);
+        if (e == cudaSuccess) e = dev::whole_smem(attend_long_kernel<T, D>);
+        if (e != cudaSuccess) return e;
+        set[device].store(true, std::memory_order_release);
+    }
     return launch_pdl(attend_long_kernel<T, D>, dim3(parts), dim3(LONG_THREADS), C::SMEM, s, maps, a);
 }
 
