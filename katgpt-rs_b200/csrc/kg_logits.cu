@@ -10,16 +10,16 @@
 // index below the cut's.
 //
 // A row is held in the shared memory of a cluster of 1 to 8 CTAs and read from
-// global memory once. A histogram of (max - x) / T in steps of 1/64, of entries and
-// for top-p of weights, says in which step each cut lies (each CTA adds up its share
-// of the steps):
+// global memory once. A histogram of (max - x) / T, of entries (in steps of 1/64) or,
+// for top-p, of entries and weights (in steps of 1/64 of an octave of w), says in which
+// step each cut lies (each CTA adds up its share of the steps):
 //   - where the candidates down to that step are at most 2048 (small top-k, a peaked
-//     row), they go to the cluster's first CTA, which finishes the row alone: it ranks
-//     up to 128 of them in both orders, or bisects their keys and indexes;
-//   - else the entries of that one step go there and the cut is bisected against the
-//     sum above them; the token is drawn by all CTAs;
-//   - where a step holds more than 2048 (rows of equal values), by bisection over the
-//     whole row.
+//     row), they go to the cluster's first CTA, which sorts them and finishes the row
+//     alone;
+//   - else the entries of that one step, at most 4096, go there and are sorted, the cut
+//     is where the running sum from what lies above them arrives; the token is drawn by
+//     all CTAs;
+//   - where a step holds more (rows of equal values), by bisection over the whole row.
 // Weights cost about 14 operations in 64 bits, which run at a half of the 32-bit
 // rate: they are computed once for top-p's histogram and once for what is drawn from.
 #include <cuda_bf16.h>
@@ -64,7 +64,7 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, RANKED = 128, LIST = 2048;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, LIST = 2048, STEP_LIST = 2 * LIST;
 constexpr int PER = LIST / THREADS;  // candidates of a thread
 
 // ---- cluster
@@ -99,54 +99,55 @@ __device__ __forceinline__ u64 remote_u64(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ void remote_store(uint32_t a, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
-__device__ __forceinline__ uint32_t remote_add(uint32_t a, uint32_t v) {
-    uint32_t r;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
-    return r;
-}
-
 struct alignas(16) Shared {
-    double tab[16];      // 2^(j / 16)
+    double tab[64];      // 2^(j / 64)
     u64 warp[2][WARPS];  // block sums
     u64 red[2][3];       // this CTA's part of what a cluster shares
-    uint32_t n_list;
+    u64 cut;             // an entry of `sorted`
+    uint32_t range[2];   // keys of a step
     uint32_t queue[WARPS][64];
     union {
         struct {
             uint32_t count[BINS], low[BINS], high[BINS];  // entries and weights (two words) of this CTA's slice by step
         };
         struct {
-            u64 list[LIST];  // key << 32 | index, of the first CTA
-            u64 order[RANKED];
-            uint32_t place[RANKED], index[RANKED];
+            u64 list[LIST];    // key << 32 | index, by index, of the first CTA
+            u64 sorted[LIST];  // key << 32 | ~index, the largest first (a step's entries: from `list` on)
         };
     };
 };
 
 static_assert(sizeof(Shared) % 16 == 0, "the keys behind it are read 16 bytes at a time");
 
-// The weight's arithmetic: 2^y by a table of 2^(j / 16), whose entries no two banks share, and the series of 2^r,
-// |r| <= 1/32 (the first term left out is below 2^-51, a hundredth of a unit). No branches: several run at a time.
+// The weight's arithmetic: 2^y by a table of 2^(j / 64) and the series of 2^r, |r| <= 1/128 (the first term left out is
+// below 2^-54). -64 y to the nearest integer is also the entry's step of the histogram. No branches: several run at a time.
 struct Weigh {
     double c, xmax;  // log2(e) / T
     uint32_t kmax;
     bool inf;
     const double *tab;
     __device__ __forceinline__ double real(uint32_t k) const {  // in units
-        const double y = ((double)value_of(k) - xmax) * c;
-        const double t = fma(y, 16.0, 6755399441055744.0);  // rounds to an integer in the low bits
+        int step;
+        return real(k, step);
+    }
+    __device__ __forceinline__ double real(uint32_t k, int &step) const {
+        if (inf) {  // (of the whole row)
+            step = k == kmax ? 0 : BINS - 1;
+            return k == kmax ? 17592186044416.0 : 0.0;
+        }
+        const double y = fmax(((double)value_of(k) - xmax) * c, -47.0);  // 2^-47 counts as 0; so does key 0, NaN
+        const double t = fma(y, 64.0, 6755399441055744.0);  // rounds to an integer in the low bits
         const int n = __double2loint(t);
-        const double r = fma(t - 6755399441055744.0, -0.0625, y);
-        double p = 0.000154035303933816061;  // ln(2)^n / n!
-        p = fma(p, r, 0.00133335581464284411);
+        const double r = fma(t - 6755399441055744.0, -0.015625, y);
+        double p = 0.00133335581464284411;  // ln(2)^n / n!
         p = fma(p, r, 0.00961812910762847688);
         p = fma(p, r, 0.0555041086648215762);
         p = fma(p, r, 0.240226506959100694);
         p = fma(p, r, 0.693147180559945286);
         p = fma(p, r, 1.0);
-        p *= tab[n & 15];
-        p = __hiloint2double(__double2hiint(p) + (((n >> 4) + 44) << 20), __double2loint(p));
-        return k == kmax ? 17592186044416.0 : !inf && y > -46.0 ? p : 0.0;  // (of key 0, NaN: 0)
+        p *= tab[n & 63];
+        step = min(-n, BINS - 1);
+        return __hiloint2double(__double2hiint(p) + (((n >> 6) + 44) << 20), __double2loint(p));
     }
     static __device__ __forceinline__ u64 whole(double w) {  // w below 2^51, to the nearest
         return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     const uint32_t rank = cluster_rank(), C = cluster_size();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = (int)rank * a.slice, n = max(0, min(a.slice, a.vocab - base));
-    if (tid < 16) sh.tab[tid] = exp2(tid / 16.0);
+    if (tid < 64) sh.tab[tid] = exp2(tid / 64.0);
     pdl_wait();
     const float T_ = a.temp ? a.temp[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const float mp = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
@@ -208,14 +209,21 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         v = lane < WARPS ? w[lane] : 0;
         return warp_sum(v);
     };
-    auto block_count = [&](uint32_t v) {
-        v = __reduce_add_sync(~0u, v);
-        u64 *w = sh.warp[flip & 1];
-        ++flip;
-        if (lane == 0) w[warp] = v;
-        __syncthreads();
-        return __reduce_add_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : 0u);
-    };
+    auto scan = [&](u64 v) {  // exclusive, over the block's threads
+                u64 x = v;
+    #pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const u64 y = __shfl_up_sync(~0u, x, d);
+                    if (lane >= d) x += y;
+                }
+                u64 *to = sh.warp[flip & 1];
+                ++flip;
+                if (lane == 31) to[warp] = x;
+                __syncthreads();
+                u64 before = 0;
+                for (int k = 0; k < warp; ++k) before += to[k];
+                return before + x - v;
+            };
     int turn = 0;
     // every CTA's values (v, x, y: the same in all its threads, or those of the thread that names them by `mine`): f(rank, v, x, y)
     auto share = [&](bool mine, u64 v, u64 x, u64 y, auto f) {
@@ -318,7 +326,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
     Weigh weigh{1.4426950408889634 / (double)T_, (double)value_of(kmax), kmax, isinf(value_of(kmax)) != 0, sh.tab};
     const double mp_units = (double)mp * 17592186044416.0;
     const float xmax = value_of(kmax), step = 64.0f / T_;
-    auto bin_of = [&](uint32_t k) { return k == kmax ? 0 : min(BINS - 1, (int)((xmax - value_of(k)) * step)); };
+    const bool has_p = p < 1.0f;
+    // an entry's step; never falls as the key falls
+    auto bin_of = [&](uint32_t k) {
+        if (has_p) {
+            int b;
+            weigh.real(k, b);
+            return b;
+        }
+        return k == kmax ? 0 : min(BINS - 1, (int)((xmax - value_of(k)) * step));
+    };
 
     uint32_t ck = 1, ci = ~0u;  // the cut
     auto stays = [&](uint32_t k, uint32_t j) { return k > ck || (k == ck && j < ci); };
@@ -348,123 +365,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         ck = c;
         ci = hi;
     };
-    // The first CTA's list, PER entries a thread in registers, and cuts of it: in the first CTA only.
-    uint32_t lk[PER], lj[PER];
-    u64 lw[PER];
-    auto list_load = [&](bool weights) {
-        const int m = (int)sh.n_list;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            const int i = tid + e * THREADS;
-            const u64 x = i < m ? sh.list[i] : 0ull;
-            lk[e] = (uint32_t)(x >> 32);
-            lj[e] = (uint32_t)x;
-            lw[e] = weights ? weigh(lk[e]) : lk[e] ? 1ull : 0ull;
-        }
-    };
-    auto list_sum = [&](auto f) {
-        u64 s = 0;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) s += f(lk[e], lj[e], lw[e]);
-        return block_sum(s);
-    };
-    auto list_count = [&](auto f) {
-        uint32_t s = 0;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) s += f(lk[e], lj[e]) ? 1u : 0u;
-        return block_count(s);
-    };
-    // the cut of the entries that stay at the first place where the sum of lw reaches `want`
-    auto list_cut = [&](u64 want, bool weights) {
-        uint32_t x = 0, y = ~0u;
-#pragma unroll
-        for (int e = 0; e < PER; ++e)
-            if (lk[e]) {
-                x = max(x, lk[e]);
-                y = min(y, lk[e]);
-            }
-        x = __reduce_max_sync(~0u, x);
-        y = __reduce_min_sync(~0u, y);
-        u64 *w = sh.warp[flip & 1];
-        ++flip;
-        if (lane == 0) w[warp] = (u64)x << 32 | y;
-        __syncthreads();
-        uint32_t hi = __reduce_max_sync(~0u, lane < WARPS ? (uint32_t)(w[lane] >> 32) : 0u);
-        uint32_t lo = __reduce_min_sync(~0u, lane < WARPS ? (uint32_t)w[lane] : ~0u);
-        constexpr int sp = Spare<T>::bits;
-        lo >>= sp;
-        hi >>= sp;
-        u64 above = 0;
-        while (lo < hi) {  // the sum over keys >= lo reaches want, that over keys > hi, `above`, does not
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
-            const u64 s = list_sum([&](uint32_t k, uint32_t j, u64 v) { return k >> sp >= mid && stays(k, j) ? v : 0ull; });
-            if (s >= want) {
-                lo = mid;
-            } else {
-                hi = mid - 1;
-                above = s;
-            }
-        }
-        const uint32_t c = key_at<T>(lo);
-        const u64 each = weights ? weigh(c) : 1ull, take = (want - above + each - 1) / each;
-        const u64 have = list_count([&](uint32_t k, uint32_t j) { return k == c && stays(k, j); });
-        uint32_t at = ck == c ? ci : ~0u;  // all of the equals that stay
-        if (take < have) {
-            uint32_t l = 0;
-            at = a.vocab;
-            while (at - l > 1) {
-                const uint32_t mid = (l + at) / 2;
-                if (list_count([&](uint32_t k, uint32_t j) { return k == c && j < mid && stays(k, j); }) >= take) at = mid;
-                else l = mid;
-            }
-        }
-        ck = c;
-        ci = at;
-    };
-    // the same, for every CTA
-    auto cut_list = [&](u64 want, bool weights) {
-        if (rank == 0) {
-            list_load(weights);
-            list_cut(want, weights);
-        }
-        u64 x = 0;
-        gather((u64)ck << 32 | ci, [&](uint32_t r, u64 v) { x = r == 0 ? v : x; });
-        ck = (uint32_t)(x >> 32);
-        ci = (uint32_t)x;
-    };
-    // live entries whose bin is in [b0, b1] and that stay, into the first CTA's list
-    auto to_list = [&](int b0, int b1) {
-        u64 in = 0;  // of this thread's entries
-        for (int i = tid * 4, e = 0; i < n; i += THREADS * 4, e += 4) {
-            const uint4 k4 = *reinterpret_cast<const uint4 *>(keys + i);
-            const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int b = bin_of(k[j]);
-                if (k[j] && b >= b0 && b <= b1 && stays(k[j], (uint32_t)(base + i + j))) in |= 1ull << (e + j);
-            }
-        }
-        if (tid == 0) sh.n_list = 0;
-        cluster_sync();  // (the histograms, which lie under the list, have been read)
-        const uint32_t mine = __popcll(in);
-        uint32_t x = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t y = __shfl_up_sync(~0u, x, d);
-            if (lane >= d) x += y;
-        }
-        uint32_t at = 0;
-        if (lane == 31 && x) at = remote_add(remote(&sh.n_list, 0), x);
-        at = __shfl_sync(~0u, at, 31) + x - mine;
-        const uint32_t dst = remote(sh.list, 0);
-        for (; in; in &= in - 1, ++at)
-            if (at < LIST) {
-                const int e = __ffsll((long long)in) - 1, i = (tid + e / 4 * THREADS) * 4 + e % 4;
-                remote_store(dst + at * 8, (u64)keys[i] << 32 | (uint32_t)(base + i));
-            }
-        __syncwarp();
-        cluster_sync();
-    };
     auto pick = [&](u64 K) {  // the place in the running sum that the given number names
         const double uu = u_in > 0.0f ? (double)u_in : 0.0;
         const u64 t = uu >= 1.0 ? K - 1 : (u64)(uu * (double)K);
@@ -475,8 +375,129 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         return t < 1.0 ? 1ull : (u64)t;
     };
 
+    // each warp looks after a run of consecutive entries of the slice
+    const int run_len = ((a.slice + WARPS - 1) / WARPS + 31) / 32 * 32, i0 = warp * run_len, i1 = min(i0 + run_len, n);
+    // The first CTA's list, in the order of the indexes, PER entries a thread in registers, and cuts of it: in the first CTA
+    // only.
+    int m_list = 0;
+    // (a pair's places lie in its warp's 64 where the stride is at most 32)
+    u64 *sorted = nullptr;
+    auto sort_list = [&](bool in_place) {
+        sorted = in_place ? sh.list : sh.sorted;
+        int N = 64;
+        while (N < m_list) N <<= 1;
+        for (int i = tid; i < N; i += THREADS) sorted[i] = i < m_list ? sh.list[i] ^ 0xffffffffull : 0ull;
+        __syncthreads();
+        for (int size = 2; size <= N; size <<= 1)
+            for (int stride = size / 2; stride; stride >>= 1) {
+                for (int q = tid; q < N / 2; q += THREADS) {
+                    const int i = 2 * q - (q & (stride - 1)), j = i + stride;
+                    const u64 x = sorted[i], y = sorted[j];
+                    if ((x < y) == ((i & size) == 0)) {
+                        sorted[i] = y;
+                        sorted[j] = x;
+                    }
+                }
+                if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads();
+                else __syncwarp();
+            }
+    };
+    auto cut_at = [&](u64 e) {  // behind entry e
+        ck = (uint32_t)(e >> 32);
+        ci = (uint32_t)~e + 1;
+    };
+    // the cut behind the first of the leading `count` sorted entries at which the sum of weights reaches part_of(W) - above
+    // (W: theirs, where `own`, of at most LIST)
+    auto cut_weights = [&](int count, bool own, u64 W, u64 above) {
+        for (int first = 0; first < count; first += LIST) {
+            u64 v[PER], here = 0;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const int i = first + tid * PER + e;
+                v[e] = i < count ? weigh((uint32_t)(sorted[i] >> 32)) : 0ull;
+                here += v[e];
+            }
+            u64 run = scan(here);
+            const u64 all = block_sum(here);
+            if (own) W = all;
+            const u64 want = part_of(W) - above;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                if (run < want && want <= run + v[e]) sh.cut = sorted[first + tid * PER + e];
+                run += v[e];
+            }
+            if (want <= all) break;
+            above += all;
+        }
+        __syncthreads();
+        cut_at(sh.cut);
+    };
+    // the first CTA's cut, for every CTA
+    auto share_cut = [&]() {
+        u64 x = 0;
+        gather((u64)ck << 32 | ci, [&](uint32_t r, u64 v) { x = r == 0 ? v : x; });
+        ck = (uint32_t)(x >> 32);
+        ci = (uint32_t)x;
+    };
+    // The smallest key whose step is at most b (32 tries at a time; the first warp).
+    auto smallest_key = [&](int b) {
+        uint32_t lo = 0x00800000u, hi = kmax;  // the answer is in [lo, hi]; lo is the key of the lowest finite value
+        while (lo < hi) {
+            const uint32_t span = (hi - lo) / 32 + 1, t = lo + lane * span < hi && lo + lane * span >= lo ? lo + lane * span : hi;
+            const uint32_t yes = __ballot_sync(~0u, bin_of(t) <= b);  // from some lane on
+            const int l = __ffs(yes) - 1;                            // (the last lane's key may be hi itself, whose step is)
+            const uint32_t at = yes ? __shfl_sync(~0u, t, l) : hi, under = yes && l == 0 ? lo : __shfl_sync(~0u, t, yes ? l - 1 : 31) + 1;
+            lo = yes && l == 0 ? at : under;
+            hi = at;
+        }
+        return hi;
+    };
+    // live entries whose bin is in [b0, b1] and that stay, into the first CTA's list
+    auto to_list = [&](int b0, int b1) {
+        if (warp == 0) {
+            const uint32_t lo = smallest_key(b1), over = b0 > 0 ? smallest_key(b0 - 1) : 0u;
+            if (lane == 0) {
+                sh.range[0] = lo;
+                sh.range[1] = b0 > 0 ? over - 1 : kmax;
+            }
+        }
+        __syncthreads();
+        const uint32_t k_lo = sh.range[0], k_hi = sh.range[1];
+        const bool whole = ck == 1;  // no cut so far
+        u64 in = 0;  // of this thread's entries of the warp's run
+        uint32_t found = 0;
+        for (int i = i0, e = 0; i < i1; i += 32, ++e) {
+            const uint32_t k = i + lane < i1 ? keys[i + lane] : 0u;
+            const bool yes = k >= k_lo && k <= k_hi && (whole || stays(k, (uint32_t)(base + i + lane)));
+            found += __popc(__ballot_sync(~0u, yes));
+            if (yes) in |= 1ull << e;
+        }
+        u64 *w = sh.warp[flip & 1];
+        ++flip;
+        if (lane == 0) w[warp] = found;
+        __syncthreads();
+        uint32_t at = 0, all = 0;
+        for (int k = 0; k < WARPS; ++k) {
+            if (k < warp) at += (uint32_t)w[k];
+            all += (uint32_t)w[k];
+        }
+        m_list = 0;
+        gather(all, [&](uint32_t r, u64 x) {  // (the histograms, which lie under the list, have been read)
+            if (r < rank) at += (uint32_t)x;
+            m_list += (int)x;
+        });
+        const uint32_t dst = remote(sh.list, 0);
+        for (int i = i0, e = 0; i < i1; i += 32, ++e) {
+            const bool yes = in >> e & 1;
+            const uint32_t who = __ballot_sync(~0u, yes);
+            const uint32_t to = at + __popc(who & ((1u << lane) - 1));
+            if (yes && to < STEP_LIST) remote_store(dst + to * 8, (u64)keys[i + lane] << 32 | (uint32_t)(base + i + lane));
+            at += __popc(who);
+        }
+        __syncwarp();
+        cluster_sync();
+    };
     const u64 kk = want_k > 0 && want_k < a.vocab ? (u64)want_k : 0ull;
-    const bool has_p = p < 1.0f;
     if (kk || has_p) {
         for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.low[i] = sh.high[i] = 0;
         __syncthreads();
@@ -487,8 +508,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
             u64 w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                b[e] = bin_of(k[e]);
-                w[e] = has_p ? weigh(k[e]) : 0ull;
+                if (has_p) {
+                    w[e] = Weigh::whole(weigh.real(k[e], b[e]));
+                } else {
+                    b[e] = bin_of(k[e]);
+                    w[e] = 0ull;
+                }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -530,21 +555,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
             c_all += c[j];
             w_all += w[j];
         }
-        auto scan = [&](u64 v) {  // exclusive, over the block's threads
-            u64 x = v;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const u64 y = __shfl_up_sync(~0u, x, d);
-                if (lane >= d) x += y;
-            }
-            u64 *to = sh.warp[flip & 1];
-            ++flip;
-            if (lane == 31) to[warp] = x;
-            __syncthreads();
-            u64 before = 0;
-            for (int k = 0; k < warp; ++k) before += to[k];
-            return before + x - v;
-        };
         u64 c_run = scan(c_all), w_run = has_p ? scan(w_all) : 0ull, live = 0, W = 0;
         share(tid == THREADS - 1, c_run + c_all, w_run + w_all, 0, [&](uint32_t r, u64 x, u64 y, u64) {
             if (r == rank) {
@@ -607,64 +617,37 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
             // Few candidates: the first CTA finishes the row.
             to_list(0, use_k ? bk : bp);
             if (rank == 0) {
-                const int m = all_of;
-                if (m <= RANKED) {
-                    u64 e = 0;
-                    if (tid < m) {
-                        e = sh.list[tid];
-                        const uint32_t k = (uint32_t)(e >> 32), j = (uint32_t)e;
-                        int ro = 0, ri = 0;
-                        for (int q = 0; q < m; ++q) {
-                            const u64 x = sh.list[q];
-                            const uint32_t xk = (uint32_t)(x >> 32), xj = (uint32_t)x;
-                            ri += xj < j;
-                            ro += xk > k || (xk == k && xj < j);
-                        }
-                        sh.order[ro] = weigh(k);
-                        sh.place[ri] = ro | (weigh.real(k) < mp_units ? 0x80000000u : 0u);
-                        sh.index[ri] = j;
-                    }
-                    __syncthreads();
-                    u64 v = tid < m && (!use_k || (u64)tid < kk) ? sh.order[tid] : 0ull;
-                    u64 run = scan(v);
-                    if (use_k) W = block_sum(v);  // what top-k leaves
-                    const u64 want = has_p ? part_of(W) : ~0ull;
-                    if (tid < m) sh.order[tid] = run < want ? v : 0ull;  // stays where what precedes it has not reached the part
-                    __syncthreads();
-                    const uint32_t q = tid < m ? sh.place[tid] : 0x80000000u;
-                    v = q & 0x80000000u ? 0ull : sh.order[q];
-                    run = scan(v);
-                    const u64 t = pick(block_sum(v));
-                    if (run <= t && t < run + v) a.out[row] = (int)sh.index[tid];
-                } else {
-                    if (use_k) {
-                        list_load(false);
-                        list_cut(kk, false);
-                    }
-                    list_load(true);
-                    if (has_p) {
-                        if (use_k) W = list_sum([&](uint32_t k, uint32_t j, u64 v) { return stays(k, j) ? v : 0ull; });
-                        list_cut(part_of(W), true);
-                    }
+                sort_list(false);
+                if (use_k) cut_at(sorted[kk - 1]);
+                if (has_p) cut_weights(use_k ? (int)kk : m_list, use_k, W, 0);
+                u64 v[PER], here = 0;
 #pragma unroll
-                    for (int e = 0; e < PER; ++e)
-                        if (!stays(lk[e], lj[e]) || weigh.real(lk[e]) < mp_units) lw[e] = 0;
-                    const u64 t = pick(list_sum([](uint32_t, uint32_t, u64 v) { return v; }));
-                    uint32_t l = 0, at = a.vocab;  // the sum over indexes below l is at most t, that below `at` exceeds it
-                    while (at - l > 1) {
-                        const uint32_t mid = (l + at) / 2;
-                        if (list_sum([&](uint32_t, uint32_t j, u64 v) { return j < mid ? v : 0ull; }) > t) at = mid;
-                        else l = mid;
-                    }
-                    if (tid == 0) a.out[row] = (int)at - 1;
+                for (int e = 0; e < PER; ++e) {
+                    const int i = tid * PER + e;
+                    const u64 x = i < m_list ? sh.list[i] : 0ull;
+                    const uint32_t k = (uint32_t)(x >> 32);
+                    const double w = weigh.real(k);
+                    v[e] = k && stays(k, (uint32_t)x) && w >= mp_units ? Weigh::whole(w) : 0ull;
+                    here += v[e];
+                }
+                u64 run = scan(here);
+                const u64 t = pick(block_sum(here));
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    if (run <= t && t < run + v[e]) a.out[row] = (int)(uint32_t)sh.list[tid * PER + e];
+                    run += v[e];
                 }
             }
             return;  // (the others' shared memory is not read any more)
         }
         if (use_k) {
-            if (n_k <= LIST) {
+            if (n_k <= STEP_LIST) {
                 to_list(bk, bk);
-                cut_list(kk - before_k, false);
+                if (rank == 0) {
+                    sort_list(true);
+                    cut_at(sorted[kk - before_k - 1]);
+                }
+                share_cut();
             } else {
                 cut_row(kk, [](uint32_t k, uint32_t) { return k ? 1ull : 0ull; }, [](uint32_t) { return 1ull; });
             }
@@ -676,9 +659,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
                 find_weight(part_of(W));
             }
             const u64 want = part_of(W);
-            if (n_p <= LIST) {
+            if (n_p <= STEP_LIST) {
                 to_list(bp, bp);
-                cut_list(want - above, true);
+                if (rank == 0) {
+                    sort_list(true);
+                    cut_weights(m_list, false, W, above);
+                }
+                share_cut();
             } else {
                 cut_row(want, f, [&](uint32_t k) { return weigh(k); });
             }
@@ -689,7 +676,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         const double w = weigh.real(k);
         return k == 0 || w < mp_units ? 0ull : Weigh::whole(w);
     };
-    const int run_len = ((a.slice + WARPS - 1) / WARPS + 31) / 32 * 32, i0 = warp * run_len, i1 = min(i0 + run_len, n);
     u64 mine = 0;
     if (ck == 1) {  // no cut
         for (int i = i0 + lane; i < i1; i += 32) mine += kept(keys[i]);
@@ -756,7 +742,7 @@ cudaError_t launch(const SampleArgs &in, cudaStream_t s) {
     // The smallest cluster whose slices stay below 16384 entries, so that two CTAs fit an SM; more CTAs where few rows
     // would leave SMs idle.
     int C = 1;
-    while (C < 8 && ((a.vocab + C - 1) / C > 16384 || ((int64_t)a.n_rows * C * 2 <= dev::sm_count() && a.vocab / C > 4096))) C *= 2;
+    while (C < 8 && ((a.vocab + C - 1) / C > 16384 || ((int64_t)a.n_rows * C <= dev::sm_count() && a.vocab / C > 4096))) C *= 2;
     a.slice = ((a.vocab + C - 1) / C + 7) / 8 * 8;
     const size_t smem = sizeof(Shared) + (size_t)a.slice * 4;
     cudaError_t e = dev::smem(sample_logits_kernel<T>, smem);
