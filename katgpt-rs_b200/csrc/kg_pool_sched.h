@@ -53,12 +53,37 @@ KG_HD int long_units(const Shape &s, int q, int kv, int i) {
     const int n = row_limit(s, q, kv, (int)(end < q ? end : q) - 1);
     return n > 0 ? (n - 1) / kLongUnit + 1 : 1;
 }
-KG_HD int64_t long_units_of_head(const Shape &s, int q, int kv) {
-    const int n = long_tiles(s, q);
-    int64_t sum = 0;
-    for (int i = 0; i < n; ++i) sum += long_units(s, q, kv, i);
-    return sum;
+// sum over i < n of floor((a i + b) / 128), a > 0, b >= 0: the terms repeat, but for a step, after 128 / gcd(a, 128)
+KG_HD int64_t sum_of_units(int n, int a, int64_t b) {
+    const int low = a & -a, period = low >= 128 ? 1 : 128 / low;
+    const int64_t rise = (int64_t)a * period / 128, rounds = n / period;
+    const int rest = n % period;
+    int64_t once = 0, tail = 0;
+    for (int i = 0; i < period && i < n; ++i) {
+        const int64_t f = ((int64_t)a * i + b) >> 7;
+        once += f;
+        if (i < rest) tail += f;
+    }
+    if (rounds == 0) return tail;
+    return rounds * once + period * rise * (rounds * (rounds - 1) / 2) + tail + rest * rounds * rise;
 }
+// units of the first n tiles of one head's long items
+KG_HD int64_t long_units_before(const Shape &s, int q, int kv, int n) {
+    const int tiles = long_tiles(s, q);
+    int64_t sum = 0;
+    if (n >= tiles && tiles > 0) {  // the last tile may be short
+        sum = long_units(s, q, kv, tiles - 1);
+        n = tiles - 1;
+    }
+    if (n <= 0) return sum;
+    if (!s.causal) return sum + (int64_t)n * long_units(s, q, kv, 0);
+    // tile i attends base + (i + 1) tile positions; where that is not positive it has one unit all the same
+    const int64_t base = (int64_t)kv - q;
+    int none = base < 0 ? (int)(-base / s.tile) : 0;
+    none = none < n ? none : n;
+    return sum + none + sum_of_units(n - none, s.tile, base + (int64_t)(none + 1) * s.tile + 127);
+}
+KG_HD int64_t long_units_of_head(const Shape &s, int q, int kv) { return long_units_before(s, q, kv, long_tiles(s, q)); }
 // units of a whole request in the line of short or of long items
 KG_HD int64_t request_units(const Shape &s, bool is_long, int q, int kv) {
     return (is_long ? long_units_of_head(s, q, kv) : short_units(s, q, kv)) * s.n_kv;
@@ -92,15 +117,16 @@ KG_HD Place place_of(const Shape &s, bool is_long, int q, int kv, int64_t off) {
     }
     const int64_t per = long_units_of_head(s, q, kv);
     p.head = (int)(off / per);
-    int64_t rest = off % per;
-    p.tile = 0;
-    while (true) {
-        p.units = long_units(s, q, kv, p.tile);
-        if (rest < p.units) break;
-        rest -= p.units;
-        ++p.tile;
+    const int64_t rest = off % per;
+    int lo = 0, hi = long_tiles(s, q) - 1;  // the last tile whose units before it are at most `rest`
+    while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (long_units_before(s, q, kv, mid) <= rest) lo = mid;
+        else hi = mid - 1;
     }
-    p.unit = (int)rest;
+    p.tile = lo;
+    p.units = long_units(s, q, kv, lo);
+    p.unit = (int)(rest - long_units_before(s, q, kv, lo));
     return p;
 }
 

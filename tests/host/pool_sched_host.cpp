@@ -66,6 +66,13 @@ int main() {
                         }
                     }
                 CHECK(off == n);
+                if (is_long) {
+                    long long sum = 0;
+                    for (int t = 0; t <= tiles; ++t) {
+                        CHECK(long_units_before(s, q[r], kv[r], t) == sum);
+                        if (t < tiles) sum += long_units(s, q[r], kv[r], t);
+                    }
+                }
                 at += n;
             }
             CHECK(at == total);

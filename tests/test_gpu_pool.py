@@ -254,6 +254,10 @@ def test_attend_layouts_and_masks(kg, be, layout, strided, causal):
     ([(90, 1000), (43, 1000), (1, 77)], 6, 2, 128, 128),   # three rows a token
     ([(70, 333), (52, 52)], 10, 2, 64, 16),                # five
     ([(2, 900)] * 40, 4, 1, 128, 16),
+    ([(70, 70)], 1, 1, 64, 16),              # fewer rows than a tile of tokens
+    ([(65, 200), (66, 65)], 2, 2, 128, 32),
+    ([(2, 50), (3, 700), (9, 130)], 64, 1, 128, 16),
+    ([(129, 20), (300, 150), (80, 0)], 2, 1, 128, 16),  # rows before position 0 in long requests
     ([(1, 130 + 3 * i) for i in range(200)], 4, 2, 64, 16),
 ])
 def test_attend_long(kg, be, reqs, n_head, n_kv, d, page):
