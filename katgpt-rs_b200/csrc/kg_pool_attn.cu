@@ -91,6 +91,8 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
         }
         *abort_flag = 0;
         mbar_fence_init();
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
     }
     // Behind the long requests' kernel this one starts as soon as that one's CTAs all run (they have waited for what came
     // before), and waits for it at its own end: the two share the device, and what follows waits for both.

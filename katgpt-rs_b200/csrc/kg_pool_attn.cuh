@@ -89,6 +89,9 @@ __device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *tm, in
         : "memory");
 }
 
+// the map itself into the loader's cache, before its first use
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *tm) { asm volatile("prefetch.tensormap [%0];" ::"l"(tm) : "memory"); }
+
 // 4-D tiled load: the rows of q of one K/V head, 64 elements wide
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *tm, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile(

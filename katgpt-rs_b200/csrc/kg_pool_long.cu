@@ -140,6 +140,9 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         }
         *abort_flag = 0;
         mbar_fence_init();
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.kv.k);
+        prefetch_map(&maps.kv.v);
     }
     pdl_wait();
     pdl_launch();  // the short requests' kernel may take the SMs that this one leaves free
