@@ -349,17 +349,37 @@ def test_attend_of_nothing(kg, be):
     _attend_case(kg, be, [(7, 0), (140, 0)], 4, 2, 64, 16, "bf16", 0)
 
 
-def test_calls_on_two_streams_and_the_current_device(kg, be):
-    """Two calls at once with a workspace each, on streams of their own."""
+def test_calls_on_two_streams(kg, be):
+    """Calls that overlap on the device, on streams of their own with a workspace each, against each of them alone."""
     import torch
-    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(7)
+    page, n_kv, d, h = 16, 2, 128, 8
+    m = torch.randn(400, 2, page, n_kv, d, generator=g, device="cuda").bfloat16()
+    pool = kg.page_pool(m.data_ptr(), m[0, 1].data_ptr(), 400, page, n_kv, d)
+    calls = []
+    for q_len, kv in (([1, 1, 3], [3000, 100, 900]), ([200, 1], [900, 400]), ([40, 33], [40, 2000])):
+        n, total = len(kv), sum(q_len)
+        table = torch.randint(0, 400, (n, 200), generator=g, device="cuda", dtype=torch.int32)
+        q = torch.randn(total, h, d, generator=g, device="cuda").bfloat16()
+        cu, kvd = _t(np.concatenate([[0], np.cumsum(q_len)])), _t(kv)
+        out = torch.zeros_like(q)
+        ws = torch.empty(be.pool_attend_bytes(pool, n, h, total), dtype=torch.uint8, device="cuda")
+        s = torch.cuda.Stream()
+
+        def call(n=n, total=total, cu=cu, kvd=kvd, table=table, q=q, out=out, ws=ws, s=s):
+            be.pool_attend_dev(pool, n, h, total, cu.data_ptr(), kvd.data_ptr(), table.data_ptr(), 200, q.data_ptr(), q.stride(0), q.stride(1),
+                               out.data_ptr(), out.stride(0), out.stride(1), d ** -0.5, 1, ws.data_ptr(), ws.numel(), s.cuda_stream)
+        torch.cuda.synchronize()
+        call()
+        torch.cuda.synchronize()
+        calls.append((call, out, out.clone()))
+    for _ in range(20):
+        for call, out, _ in calls:
+            call()
     torch.cuda.synchronize()
-    with torch.cuda.stream(a):
-        x = _attend_case(kg, be, [(1, 3000)], 8, 2, 128, 16, "bf16", 1, seed=11, stream=a.cuda_stream)
-    with torch.cuda.stream(b):
-        y = _attend_case(kg, be, [(200, 900)], 8, 2, 128, 16, "bf16", 1, seed=12, stream=b.cuda_stream)
-    np.testing.assert_array_equal(x, _attend_case(kg, be, [(1, 3000)], 8, 2, 128, 16, "bf16", 1, seed=11))
-    np.testing.assert_array_equal(y, _attend_case(kg, be, [(200, 900)], 8, 2, 128, 16, "bf16", 1, seed=12))
+    be.pool_status()
+    for _, out, alone in calls:
+        assert torch.equal(out, alone)
 
 
 # ---------------------------------------------------------------- together

@@ -1,6 +1,8 @@
 """Refusals of the serving operators over a caller-owned page pool: every check of arguments runs before the
 context is used, so a null context shows them without a device (kg_last_error(NULL) has the message)."""
 import ctypes
+import os
+import re
 
 import pytest
 
@@ -161,6 +163,15 @@ def test_sample_refusals(kg, kw, code, text):
     a = dict(n_rows=3, vocab=100, dtype=0, logits=A16, ld=100, t=A16, k=A16, p=A16, m=A16, u=A16, out=A16)
     a.update(kw)
     _refused(kg, kg.lib().kg_sample_logits_dev(None, *a.values(), None), code, text)
+
+
+def test_pool_mirrors_have_the_headers_fields(kg):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    header = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "kg_abi.h")).read(), flags=re.S)
+    fields = re.findall(r"\b(\w+)\s*;", re.search(r"typedef struct \{([^}]*)\}\s*kg_pool;", header).group(1))
+    assert fields == [f for f, _ in kg.KgPool._fields_]
+    rust = re.search(r"pub struct KgPool \{([^}]*)\}", open(os.path.join(root, "INTEGRATION.md")).read()).group(1)
+    assert re.findall(r"pub (\w+):", rust) == fields
 
 
 def test_attend_bytes_raises_in_python(kg):
