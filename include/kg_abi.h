@@ -306,20 +306,22 @@ int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const in
  * positions up to its own, otherwise all kv_len[r] of them (as forward_prefill
  * does over its prompt). Query head h reads KV head h / (n_head / n_kv_head):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]
- * (scale not negative) with f32 scores, statistics and sums; a row that attends nothing (kv_len 0,
- * or a row before position 0) becomes zeros. The probabilities enter the second
- * product in the pool's type, everything is rounded once at the end. q and out
- * have the pool's type, out row i head h at i * out_row_stride + h *
- * out_head_stride; q and out must not overlap. Rows outside every request's
- * range are left as they were. Page contents past kv_len are never used; those
- * before it are finite. Device-side checks: cu_q non-decreasing within [0,
- * total_q], kv_len within [0, table_width * page_size] and below 2^31 - 256, or
- * the request's rows are left as they were; a table entry outside the pool reads as zeros; either
- * is reported. n_head at most 64 times n_kv_head, at most 16384 requests.
- * workspace: kg_pool_attend_bytes() bytes (80 MB at most), 16-byte aligned, for partial results
- * when one request's positions are split over several CTAs; its content need
- * not be kept or initialised, and calls that may overlap on the device (other
- * streams, two graphs) need one each. kg_pool_attend_bytes returns a negative
+ * (scale not negative) with f32 scores, statistics and sums; a row that attends
+ * nothing (kv_len 0, or a row before position 0) becomes zeros. The probabilities
+ * enter the second product in the pool's type, everything is rounded once at the
+ * end. The same call gives the same bits; how a request's sums are cut, and with
+ * it their last bits, depends on the batch that it is in. q and out have the pool's
+ * type, out row i head h at i * out_row_stride + h * out_head_stride; q and out must
+ * not overlap. Rows outside every request's range are left as they were. Page
+ * contents past kv_len are never used; those before it are finite. Device-side
+ * checks: cu_q non-decreasing within [0, total_q], kv_len within [0, table_width *
+ * page_size] and below 2^31 - 256, or the request's rows are left as they were; a
+ * table entry outside the pool reads as zeros; either is reported. n_head at most
+ * 64 times n_kv_head, at most 16384 requests.
+ * workspace: kg_pool_attend_bytes() bytes (77 MB at most), 16-byte aligned, for
+ * partial results when one request's positions are split over several CTAs; its
+ * content need not be kept or initialised, and calls that may overlap on the device
+ * (other streams, two graphs) need one each. kg_pool_attend_bytes returns a negative
  * kg_status for arguments that kg_pool_attend_dev refuses. */
 int64_t kg_pool_attend_bytes(const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q);
 int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q,

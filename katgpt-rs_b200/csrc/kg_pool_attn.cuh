@@ -112,33 +112,39 @@ __device__ __forceinline__ bool req_len(const AttendArgs &a, int r, int &q0, int
     return ok;
 }
 
-// This CTA's part: where it begins and how many units it has. At most `parts`
-// parts of at least `least` units. Every thread of the block calls it (NT
-// threads); `sm` holds NT / 32 + 2 numbers.
+// This CTA's part (of parts_of() ones): where it begins and how many units it has.
+// Every thread of the block calls it (NT threads); `sm` holds 2 NT / 32 + 2 numbers.
 template <int NT, bool LONG>
 __device__ void find_part(const AttendArgs &a, int c, int parts, int least, long long *sm, int &req, long long &off,
                           long long &units) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.n_req + NT - 1) / NT, r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
-    long long mine = 0;
+    long long mine = 0, items = 0;
     for (int r = r0; r < r1; ++r) {
         int q0, q, kv;
         if (!req_len(a, r, q0, q, kv) && c == 0) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
         mine += request_units(a.s, LONG, q, kv);
+        items += request_items(a.s, LONG, q, kv);
     }
     long long incl = mine;
     for (int d = 1; d < 32; d <<= 1) {
         const long long u = __shfl_up_sync(~0u, incl, d);
         if (lane >= d) incl += u;
     }
-    if (lane == 31) sm[warp] = incl;
+    const int few = __reduce_add_sync(~0u, (int)min(items, 65536ll));  // enough to compare with the CTAs there are
+    if (lane == 31) {
+        sm[warp] = incl;
+        sm[NT / 32 + warp] = few;
+    }
     __syncthreads();
     long long before = incl - mine, total = 0;
+    items = 0;
     for (int w = 0; w < NT / 32; ++w) {
         if (w < warp) before += sm[w];
         total += sm[w];
+        items += sm[NT / 32 + w];
     }
-    parts = (int)min((long long)parts, (total + least - 1) / least);
+    parts = parts_of(total, items, parts, least);
     const long long b = c < parts ? part_begin(total, c, parts) : 0, e = c < parts ? part_begin(total, c + 1, parts) : 0;
     units = e - b;
     if (units > 0 && before <= b && b < before + mine) {
@@ -148,16 +154,16 @@ __device__ void find_part(const AttendArgs &a, int c, int parts, int least, long
             req_len(a, r, q0, q, kv);
             const long long n = request_units(a.s, LONG, q, kv);
             if (b < at + n) {
-                sm[NT / 32] = r;
-                sm[NT / 32 + 1] = b - at;
+                sm[2 * (NT / 32)] = r;
+                sm[2 * (NT / 32) + 1] = b - at;
                 break;
             }
             at += n;
         }
     }
     __syncthreads();
-    req = units > 0 ? (int)sm[NT / 32] : 0;
-    off = units > 0 ? sm[NT / 32 + 1] : 0;
+    req = units > 0 ? (int)sm[2 * (NT / 32)] : 0;
+    off = units > 0 ? sm[2 * (NT / 32) + 1] : 0;
 }
 
 // The items of a part, in order.

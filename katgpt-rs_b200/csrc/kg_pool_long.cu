@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     uint64_t *sfull = qempty + 1, *pvdone = sfull + 2, *pready = pvdone + 2;  // [2] by tile, pready [tile][half]
     uint32_t *tslot = reinterpret_cast<uint32_t *>(pready + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tslot + 1);
-    __shared__ long long part_sm[LONG_THREADS / 32 + 2];
+    __shared__ long long part_sm[2 * (LONG_THREADS / 32) + 2];
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, c = blockIdx.x;
     const int group = a.s.group, tq = a.s.tile / 2;
     if (threadIdx.x == 0) {

@@ -88,6 +88,16 @@ KG_HD int64_t long_units_of_head(const Shape &s, int q, int kv) { return long_un
 KG_HD int64_t request_units(const Shape &s, bool is_long, int q, int kv) {
     return (is_long ? long_units_of_head(s, q, kv) : short_units(s, q, kv)) * s.n_kv;
 }
+// items of a request
+KG_HD int64_t request_items(const Shape &s, bool is_long, int q, int kv) {
+    return (is_long ? long_tiles(s, q) : q > 0 && is_short(s, q) ? 1 : 0) * (int64_t)s.n_kv;
+}
+// Parts of a line: at most `most`, of at least `least` units each, but one for every item where there are so few (a CTA
+// takes its items one after the other).
+KG_HD int parts_of(int64_t units, int64_t items, int most, int least) {
+    const int64_t n = (units + least - 1) / least, m = n > items ? n : items;
+    return (int)(m < most ? m : most);
+}
 // the first unit of part c of `parts` (in 32 bits where they suffice: 64-bit divisions are slow on the device)
 KG_HD int64_t part_begin(int64_t units, int c, int parts) {
     if (units <= 4194303) {  // units % parts * c stays below 512 * 512
