@@ -20,6 +20,8 @@
 //     is where the running sum from what lies above them arrives; the token is drawn by
 //     all CTAs;
 //   - where a step holds more (rows of equal values), by bisection over the whole row.
+// Bound by the latency of a row's steps: 64 rows of 32000 in 44 us, 256 nucleus rows of
+// 131072 in 500 us (33 clusters at a time, about 50 us a row; read alone, 10 us).
 // Weights cost about 14 operations in 64 bits, which run at a half of the 32-bit
 // rate: they are computed once for top-p's histogram and once for what is drawn from.
 #include <cuda_bf16.h>

@@ -27,7 +27,9 @@ namespace {
 // token t to the request whose token range holds t.
 // Bound by latency: one launch. A cluster of 1 or 8 CTAs; each computes the running
 // sums for itself (a few loads a thread), the checks meet at a cluster barrier
-// before anything is written, and the tokens and pages are shared out.
+// before anything is written, and the tokens and pages are shared out. 512 ragged
+// requests of 64 K tokens: 77 us by one CTA, 12.4 us a call by eight; 64 single tokens:
+// 9.7 us a call, the host's time.
 struct PlanArgs {
     int page, n_pages, n_req, width, max_tokens;
     const int32_t *cached, *fresh;
@@ -187,7 +189,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Store: one thread moves eight elements of one row, K or V.
+// Store: one thread moves eight elements of one row, K or V: 16 bytes written, 16 or
+// 32 read, neighbours side by side on both sides. Bound by HBM: 16,500 f32 rows of 12
+// heads of 64, 151 MB, in 27 us (85% of the copy rate).
 struct StoreArgs {
     kg_pool p;
     const void *k, *v;
@@ -294,6 +298,7 @@ int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const in
     if (n_rows < 0) return fail(ctx, KG_ERR_INVALID_ARG, "store: n_rows must not be negative");
     if (src_dtype != KG_DT_F32 && src_dtype != KG_DT_BF16 && src_dtype != KG_DT_F16)
         return fail(ctx, KG_ERR_UNSUPPORTED, "store: src_dtype must be KG_DT_F32, KG_DT_BF16 or KG_DT_F16");
+    if ((int64_t)n_rows * pool->n_kv_head > INT32_MAX) return fail(ctx, KG_ERR_UNSUPPORTED, "store: too many rows (n_rows * n_kv_head)");
     if (n_rows > 0) {
         if (!slots || !k || !v) return fail(ctx, KG_ERR_INVALID_ARG, "store: null pointer");
         const int unit = src_dtype == KG_DT_F32 ? 4 : 8;

@@ -200,7 +200,9 @@ def _attend_case(kg, be, reqs, n_head, n_kv, d, page, dt, causal, layout="page",
     total = int(cu[-1]) + pad
     q = torch.from_numpy(rng.standard_normal((total, n_head, d))).mul(spread).to(td)
     scale = d ** -0.5
-    if strided:  # q inside a fused projection's rows, out with heads first
+    if strided == "heads first":
+        qd, out = q.transpose(0, 1).contiguous().cuda().transpose(0, 1), torch.full((total, n_head, d), 7.0, dtype=td, device="cuda")
+    elif strided:  # q inside a fused projection's rows, out with heads first
         big = torch.zeros(total, n_head + 2 * n_kv, d, dtype=td)
         big[:, :n_head] = q
         qd = big.cuda()[:, :n_head]
@@ -240,7 +242,7 @@ def test_attend_head_layouts(kg, be, n_head, n_kv):
     _attend_case(kg, be, [(1, 300), (9, 70), (1, 1), (40, 200)], n_head, n_kv, 64, 16, "bf16", 1, pad=1, seed=n_head)
 
 
-@pytest.mark.parametrize("layout,strided,causal", list(itertools.product(LAYOUTS, [False, True], [0, 1])))
+@pytest.mark.parametrize("layout,strided,causal", list(itertools.product(LAYOUTS, [False, True, "heads first"], [0, 1])))
 def test_attend_layouts_and_masks(kg, be, layout, strided, causal):
     _attend_case(kg, be, [(1, 90), (33, 50), (4, 3), (20, 260)], 6, 2, 128, 16, "bf16", causal, layout=layout, strided=strided, seed=9)
 
@@ -254,6 +256,8 @@ def test_attend_layouts_and_masks(kg, be, layout, strided, causal):
     ([(90, 1000), (43, 1000), (1, 77)], 6, 2, 128, 128),   # three rows a token
     ([(70, 333), (52, 52)], 10, 2, 64, 16),                # five
     ([(2, 900)] * 40, 4, 1, 128, 16),
+    ([(20, 9000)], 8, 1, 128, 16),           # one tile's positions split over many CTAs
+    ([(1, 70001), (1, 3)], 2, 1, 64, 128),
     ([(70, 70)], 1, 1, 64, 16),              # fewer rows than a tile of tokens
     ([(65, 200), (66, 65)], 2, 2, 128, 32),
     ([(2, 50), (3, 700), (9, 130)], 64, 1, 128, 16),

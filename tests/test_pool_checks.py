@@ -73,11 +73,12 @@ def test_null_pool_and_context(kg):
     (dict(rs=130), INVALID, "aligned"),
     (dict(src=1, rs=132), INVALID, "aligned"),
     (dict(hs=-64), INVALID, "aligned"),
+    (dict(n_rows=2**31 - 1, pool=dict(n_kv_head=1024, row_stride=1024 * 64, page_stride=1 << 21)), UNSUPPORTED, "too many rows"),
 ])
 def test_store_refusals(kg, kw, code, text):
-    a = dict(n_rows=4, slots=A16, src=0, k=A16, v=A16, rs=128, hs=64)
+    a = dict(n_rows=4, slots=A16, src=0, k=A16, v=A16, rs=128, hs=64, pool={})
     a.update(kw)
-    rc = kg.lib().kg_pool_store_dev(None, _pool(kg), a["n_rows"], a["slots"], a["src"], a["k"], a["v"], a["rs"], a["hs"], None)
+    rc = kg.lib().kg_pool_store_dev(None, _pool(kg, **a["pool"]), a["n_rows"], a["slots"], a["src"], a["k"], a["v"], a["rs"], a["hs"], None)
     _refused(kg, rc, code, text)
 
 
