@@ -94,13 +94,14 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t a) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ int pack_bits(u64 v, int at, int bits) { return (int)(v >> at & ((1ull << bits) - 1)); }
+__device__ __forceinline__ int bits_of(u64 v, int at, int bits) { return (int)(v >> at & ((1ull << bits) - 1)); }
 __device__ __forceinline__ u64 remote_u64(uint32_t a) {
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
     return v;
 }
 __device__ __forceinline__ void remote_store(uint32_t a, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
+
 struct alignas(16) Shared {
     double tab[64];      // 2^(j / 64)
     u64 warp[2][WARPS];  // block sums
@@ -379,10 +380,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
 
     // each warp looks after a run of consecutive entries of the slice
     const int run_len = ((a.slice + WARPS - 1) / WARPS + 31) / 32 * 32, i0 = warp * run_len, i1 = min(i0 + run_len, n);
-    // The first CTA's list, in the order of the indexes, PER entries a thread in registers, and cuts of it: in the first CTA
-    // only.
+    // The first CTA's list (m_list entries in the order of the indexes), sorted by key and index: in the first CTA only. A
+    // pair's places lie in its warp's 64 where the stride is at most 32.
     int m_list = 0;
-    // (a pair's places lie in its warp's 64 where the stride is at most 32)
     u64 *sorted = nullptr;
     auto sort_list = [&](bool in_place) {
         sorted = in_place ? sh.list : sh.sorted;
@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         __syncwarp();
         cluster_sync();
     };
+
     const u64 kk = want_k > 0 && want_k < a.vocab ? (u64)want_k : 0ull;
     if (kk || has_p) {
         for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.low[i] = sh.high[i] = 0;
@@ -581,9 +582,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
             __syncthreads();
             u64 got = 0;
             share(hit != 0, hit, 0, 0, [&](uint32_t, u64 v, u64, u64) { got = max(got, v); });
-            bk = pack_bits(got, 40, 12);
-            before_k = pack_bits(got, 20, 20);
-            n_k = pack_bits(got, 0, 20);
+            bk = bits_of(got, 40, 12);
+            before_k = bits_of(got, 20, 20);
+            n_k = bits_of(got, 0, 20);
         }
         // The step that holds the place where the weights reach `want` (among the first bk, or bk itself).
         u64 above = 0;
@@ -609,9 +610,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
                     above = ab;
                 }
             });
-            bp = pack_bits(got, 40, 12);
-            before_p = pack_bits(got, 20, 20);
-            n_p = pack_bits(got, 0, 20);
+            bp = bits_of(got, 40, 12);
+            before_p = bits_of(got, 20, 20);
+            n_p = bits_of(got, 0, 20);
         };
         if (!use_k && has_p) find_weight(part_of(W));
         const int all_of = use_k ? before_k + n_k : before_p + n_p;
