@@ -308,8 +308,8 @@ int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const in
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]
  * (scale not negative) with f32 scores, statistics and sums; a row that attends
  * nothing (kv_len 0, or a row before position 0) becomes zeros. The probabilities
- * enter the second product in the pool's type, everything is rounded once at the
- * end. The same call gives the same bits; how a request's sums are cut, and with
+ * enter the second product in the pool's type (in f16 those below 2^-26 of a row's
+ * largest lose bits, those below 2^-36 are 0), everything is rounded once at the end. The same call gives the same bits; how a request's sums are cut, and with
  * it their last bits, depends on the batch that it is in. q and out have the pool's
  * type, out row i head h at i * out_row_stride + h * out_head_stride; q and out must
  * not overlap. Rows outside every request's range are left as they were. Page

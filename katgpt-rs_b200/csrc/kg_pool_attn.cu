@@ -1,7 +1,8 @@
 // kg_pool_attn.cu — kg_pool_attend_dev: attention of new rows over a paged K/V
 // pool, ragged over requests.
 //
-// One pass over the positions with a running maximum m and sum l per row:
+// One pass over the positions with a running maximum m (less a constant in f16: Cvt) and
+// sum l per row:
 //   o = sum_j 2^(s_j - m) v_j,  l = sum_j 2^(s_j - m),  s_j = scale log2(e) q.k_j
 // A part of the positions gives (o, m, l); parts of one item join as
 //   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                         }
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                    const float mn = fmaxf(m[i], mx);
+                    const float mn = fmaxf(m[i], base_of(mx, Cvt<T>::UP));
                     if (__any_sync(~0u, mn != m[i])) {
                         const float f = mn == -INFINITY ? 1.0f : exp2_approx(m[i] - mn);
                         l[i] *= f;

@@ -17,8 +17,9 @@
 // 555 us under the power cap (1,030 to 1,200 TFLOP/s). A pair of units takes about 3,150
 // cycles, of which the products 2,055 and the exponentials 2,048 run beside each other:
 // bound by the chain scores -> exponentials -> values -> next scores of one tile.
-// A row's O is rescaled only when its maximum has grown by more than 2^8 since the
-// last time: P then reaches at most 2^8, which 16 bits hold as exactly as 1.
+// A row's O is rescaled only when its maximum has grown by more than 2^LAG since the
+// last time: 2^8 in bf16, whose P then reaches at most 2^8; 2^3 in f16, whose P has to
+// use the range that it has (Cvt).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -40,7 +41,6 @@ namespace {
 using namespace as;
 
 constexpr int LONG_THREADS = 320, LONG_LEAST = 2;
-constexpr float RESCALE = 8.0f;
 
 template <int D>
 struct LongCfg {
@@ -337,12 +337,14 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 half(0);
                 top = fmaxf(top, top_of());
                 top = top == -INFINITY ? top : top * a.scale;
-                const bool grow = u == 0 || top > m + RESCALE;
+                const bool grow = u == 0 || top - m > Cvt<T>::UP_LONG + Cvt<T>::LAG;
                 if (u == 0) {
-                    m = top;
+                    m = base_of(top, Cvt<T>::UP_LONG);
                 } else if (__any_sync(~0u, grow)) {
-                    const float f = grow ? exp2_approx(m - top) : 1.0f;
-                    if (grow) m = top;
+                    // (in f16, which has little room, every row of the warp whose maximum has grown joins in)
+                    const bool up = Cvt<T>::UP_LONG > 0.0f ? top - m > Cvt<T>::UP_LONG : grow;
+                    const float next = base_of(top, Cvt<T>::UP_LONG), f = up ? exp2_approx(m - next) : 1.0f;
+                    if (up) m = next;
                     l *= f;
                     ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
                     if (!ok) break;

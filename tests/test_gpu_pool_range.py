@@ -1,0 +1,88 @@
+"""Attention over the page pool where the numbers' range counts: probabilities far below a row's largest, which f16 holds
+only near its own upper end, and scores so large that f32 has no number near them. Against 64 bits, in both kernels
+(requests of at most 64 rows a K/V head, and longer ones)."""
+import numpy as np
+import pytest
+
+import pool_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be(kg):
+    b = kg.CudaBackend(kg.micro_config())
+    yield b
+    b.pool_status()
+    b.close()
+
+
+def _shared(kg, be, k, v, q, n_req, dt, scale, causal, page=64):
+    """`n_req` requests of q's rows each over the same pages: (rows of all requests, their 64-bit values, tolerances).
+    k, v: [positions][kv heads][d], q: [rows][heads][d], numpy."""
+    import torch
+    td = {"bf16": torch.bfloat16, "f16": torch.float16}[dt]
+    kv, n_kv, d = k.shape
+    rows, heads, _ = q.shape
+    pages = -(-kv // page)
+    m = torch.full((pages, 2, page, n_kv, d), float("nan"), dtype=td, device="cuda")
+    for i, x in enumerate((k, v)):
+        y = torch.full((pages * page, n_kv, d), float("nan"), dtype=td)
+        y[:kv] = torch.from_numpy(x).to(td)
+        m[:, i] = y.view(pages, page, n_kv, d).cuda()
+    k, v, q = (torch.from_numpy(x).to(td) for x in (k, v, q))
+    pool = kg.page_pool(m.data_ptr(), m[0, 1].data_ptr(), pages, page, n_kv, d, dt)
+    qd = q.cuda().repeat(n_req, 1, 1)
+    out = torch.full_like(qd, 7.0)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cu, kvd = torch.arange(n_req + 1, **i32) * rows, torch.full((n_req,), kv, **i32)
+    table = torch.arange(pages, **i32).repeat(n_req, 1)
+    ws = torch.full((be.pool_attend_bytes(pool, n_req, heads, n_req * rows),), 0xFF, dtype=torch.uint8, device="cuda")
+    be.pool_attend_dev(pool, n_req, heads, n_req * rows, cu.data_ptr(), kvd.data_ptr(), table.data_ptr(), pages, qd.data_ptr(), qd.stride(0),
+                       qd.stride(1), out.data_ptr(), out.stride(0), out.stride(1), scale, causal, ws.data_ptr(), ws.numel())
+    torch.cuda.synchronize()
+    be.pool_status()
+    want, _, mag, sco = po.attend(q.double().numpy(), [k.double().numpy()], [v.double().numpy()], [0, rows], [kv], scale, causal)
+    # one rounding of the result and one of every probability, half a step each, f32 scores (d products) and 2^-18 for exp
+    # and the running sums, as for ordinary batches
+    half = torch.finfo(td).eps / 2
+    tol = half * np.abs(want) * 1.01 + mag * (half * 1.01 + 2 * d * 2.0 ** -24 * sco[..., None] + 2.0 ** -18) + 2.0 ** -24
+    return out.double().cpu().numpy().reshape(n_req, rows, heads, d), want, tol
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n_req,positions,nats,d", [
+    (1, 1, 65536, 17.3, 64), (5, 1, 16384, 16.2, 128), (1, 300, 2000, 15.0, 128), (4, 9, 3001, 17.0, 64),  # short
+    (40, 1, 65536, 17.3, 64), (150, 1, 16384, 16.2, 128), (40, 80, 2000, 15.0, 128), (70, 9, 3001, 17.0, 64),  # long
+])
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+def test_a_far_peak_and_a_flat_rest(kg, be, dt, rows, n_req, positions, nats, d, at):
+    """One position takes nearly the whole weight and has no value (an attention sink); the result is the flat rest's share,
+    whose probabilities lie 2^-21 to 2^-25 below the largest."""
+    rng = np.random.default_rng(rows + positions)
+    k, v = np.zeros((positions, 1, d)), rng.uniform(0.5, 1.5, (positions, 1, d))
+    peak = {"first": 0, "middle": positions // 2, "last": positions - rows}[at]  # every row attends it
+    k[peak, 0, 0], v[peak] = nats * d ** 0.5 / 8, 0.0
+    q = rng.standard_normal((rows, 2, d))
+    q[..., 0] = 8.0
+    got, want, tol = _shared(kg, be, k, v, q, n_req, dt, d ** -0.5, 1)
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_past_the_whole_numbers_of_f32(kg, be, dt, rows, sign):
+    """Equal scores of 2^18 to 2^29: every weight is the same, whatever is subtracted from the scores must not make one
+    of them overflow."""
+    d, positions = 64, 300
+    rng = np.random.default_rng(5)
+    v = rng.uniform(0.5, 1.5, (positions, 1, d))
+    q = np.zeros((rows, 1, d))
+    q[..., 0] = 2.0 ** 14
+    for e in range(4, 16):
+        for f in (1.0, 1.375):
+            k = np.zeros((positions, 1, d))
+            k[..., 0] = sign * f * 2.0 ** e
+            got, want, tol = _shared(kg, be, k, v, q, 1, dt, 1.0, 0)
+            assert (np.abs(got - want) <= tol).all(), (e, f)
