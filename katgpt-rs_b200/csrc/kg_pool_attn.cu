@@ -147,6 +147,8 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     }
 
     const int gid = lane >> 2, tig = lane & 3;
+    Ring ring{full, empty, abort_flag, a.err};
+    bool ok = true;
     int it = 0;
     do {
         const int rows = w.q * a.s.group, wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;  // row groups
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
         for (int u = 0; u < w.n; ++u, ++it) {
             const int s = it % C::STAGES;
             // (a wait that gave up skips the work, not the barriers below)
-            const bool ok = mbar_wait(&full[s], (it / C::STAGES) & 1, abort_flag, a.err);
+            ok = ring_take(ring, C::STAGES, it, ok);
             uint8_t *st = sm + s * 2 * C::OP_BYTES;
             bool wrote = false;
             const int chunk = C::UNIT / 4 * wm, p_end = (pg + 1) * chunk, unit0 = (w.p.unit + u) * C::UNIT;

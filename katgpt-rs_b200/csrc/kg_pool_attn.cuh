@@ -8,7 +8,7 @@
 #include <cuda_runtime.h>
 
 #include "kg_async.cuh"
-#include "kg_pool_sched.h"
+#include "kg_pool_ring.h"
 
 namespace kg {
 namespace serve {
@@ -71,6 +71,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// The barriers of a ring of stages (kg_pool_ring.h).
+struct Ring {
+    uint64_t *full, *empty;
+    volatile int *abort_flag;
+    int *err;
+    __device__ __forceinline__ bool wait_full(int s, int parity) { return as::mbar_wait(&full[s], parity, abort_flag, err); }
+    __device__ __forceinline__ bool all(bool x) { return __all_sync(~0u, x) != 0; }
+};
 
 // A producer that gave up on a wait: its loads in flight end before the block's shared memory is given back (each wait
 // bounded again). `it` loads were issued into a ring of `stages`.
