@@ -113,12 +113,14 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     Walk<false> w;
     w.start(a, req, off, units);
 
+    Ring ring{full, empty, 2 * C::OP_BYTES, abort_flag, a.err};
     if (warp == 4) {  // producer: lane i loads box i of a unit
         const int rows = min(a.page_size, kBoxRows), pages = C::UNIT / rows, boxes = pages * 2;
         const int piece = lane % pages, which = lane / pages;
         const CUtensorMap *tm = which ? &maps.v : &maps.k;
         const int dst = which * C::OP_BYTES + piece * rows * D * 2;
         int it = 0;
+        bool ok = true;
         do {
             for (int u = 0; u < w.n; ++u, ++it) {
                 const int s = it % C::STAGES, pos = (w.p.unit + u) * C::UNIT + piece * rows;
@@ -128,26 +130,19 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                     if (e >= 0 && e < a.n_pages) place = e * maps.page_step + w.p.head * maps.head_step;
                     else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
                 }
-                int ok = 1;
-                if (lane == 0) {
-                    ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, a.err);
-                    if (ok) mbar_expect_tx(&full[s], 2 * C::OP_BYTES);
-                }
-                if (!__shfl_sync(~0u, ok, 0)) {
-                    drain_loads(full, C::STAGES, it);
-                    if (after_long) pdl_wait();
-                    return;
-                }
+                if (lane == 0) ok = ring_claim(ring, C::STAGES, it);
+                ok = __shfl_sync(~0u, ok, 0);
+                if (!ok) break;
                 if (lane < boxes)
                     tma_load_5d(sm + s * 2 * C::OP_BYTES + dst, tm, pos % a.page_size / 8, place, &full[s]);
             }
-        } while (w.next(a));
+        } while (ok && w.next(a));
+        ring_drain(ring, C::STAGES, it);
         if (after_long) pdl_wait();
         return;
     }
 
     const int gid = lane >> 2, tig = lane & 3;
-    Ring ring{full, empty, abort_flag, a.err};
     bool ok = true;
     int it = 0;
     do {
@@ -261,7 +256,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
             }
             if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the stage again
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[s]);
+            if (lane == 0) ring_free(ring, C::STAGES, it, ok);
         }
         // join the warps that share rows and write the item
 #pragma unroll

@@ -72,24 +72,25 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// The barriers of a ring of stages (kg_pool_ring.h).
+// The barriers of a ring of stages (kg_pool_ring.h), `bytes` in each.
 struct Ring {
     uint64_t *full, *empty;
+    uint32_t bytes;
     volatile int *abort_flag;
     int *err;
     __device__ __forceinline__ bool wait_full(int s, int parity) { return as::mbar_wait(&full[s], parity, abort_flag, err); }
+    __device__ __forceinline__ bool wait_empty(int s, int parity) { return as::mbar_wait(&empty[s], parity, abort_flag, err); }
+    __device__ __forceinline__ void arm(int s) { as::mbar_expect_tx(&full[s], bytes); }
+    __device__ __forceinline__ void free(int s) { as::mbar_arrive(&empty[s]); }
     __device__ __forceinline__ bool all(bool x) { return __all_sync(~0u, x) != 0; }
-};
-
-// A producer that gave up on a wait: its loads in flight end before the block's shared memory is given back (each wait
-// bounded again). `it` loads were issued into a ring of `stages`.
-__device__ __forceinline__ void drain_loads(uint64_t *full, int stages, int it) {
-    for (int i = it > stages ? it - stages : 0; i < it; ++i) {
+    // a load that has been issued ends whatever else happened (bounded all the same)
+    __device__ __forceinline__ void landed(int s, int parity) { wait_landed(&full[s], parity); }
+    static __device__ __forceinline__ void wait_landed(uint64_t *bar, int parity) {
         const long long t0 = clock64();
-        while (!as::mbar_try(&full[i % stages], (i / stages) & 1) && clock64() - t0 < (1ll << 28)) {
+        while (!as::mbar_try(bar, parity) && clock64() - t0 < (1ll << 28)) {
         }
     }
-}
+};
 
 // Shared-memory form of K and V: groups of 8 positions, each [head_dim / 64][8
 // rows][128 bytes] with the 128-byte swizzle. One TMA box brings all of a page's

@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     using C = LongCfg<D>;
     extern __shared__ __align__(1024) uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (sa(raw) & 1023u)) & 1023u);
-    uint8_t *sq = sm, *ring = sm + 2 * C::OP;
-    uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::SLOTS * C::OP), *empty = full + C::SLOTS;
+    uint8_t *sq = sm, *slots = sm + 2 * C::OP;
+    uint64_t *full = reinterpret_cast<uint64_t *>(slots + C::SLOTS * C::OP), *empty = full + C::SLOTS;
     uint64_t *qfull = empty + C::SLOTS, *qempty = qfull + 1;
     uint64_t *sfull = qempty + 1, *pvdone = sfull + 2, *pready = pvdone + 2;  // [2] by tile, pready [tile][half]
     uint32_t *tslot = reinterpret_cast<uint32_t *>(pready + 4);
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         return max(0, min(w.n, u - w.p.unit));
     };
 
+    Ring ring{full, empty, C::OP, abort_flag, a.err};
     if (warp == 0) {  // loads
         const int rows = min(a.page_size, kBoxRows), pages = kLongUnit / rows;  // a box each
         int it = 0, item = 0;
@@ -204,12 +205,12 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     }
                     ok = __shfl_sync(~0u, ok, 0);
                     if (ok && lane < pages)
-                        tma_load_5d(ring + s * C::OP + lane * rows * D * 2, kv ? &maps.kv.v : &maps.kv.k, pos % a.page_size / 8, place, &full[s]);
+                        tma_load_5d(slots + s * C::OP + lane * rows * D * 2, kv ? &maps.kv.v : &maps.kv.k, pos % a.page_size / 8, place, &full[s]);
                 }
             }
             ++item;
         } while (ok && w.next(a));
-        if (!ok) drain_loads(full, C::SLOTS, it);
+        if (!ok) ring_drain(ring, C::SLOTS, it);
     } else if (warp == 1) {  // products, tile 0 and tile 1 in turn
         // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers. From inside a
         // one-lane branch a product took about 110 cycles to issue, against 64 to run.
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             auto wait = [&](uint64_t *b, int parity) { return __all_sync(~0u, mbar_wait(b, parity, abort_flag, a.err)) != 0; };
             auto wait_slot = [&](int step) { return wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1); };
             auto scores = [&](int t, int step) {
-                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), 16, D * 16);
+                const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_sw128(sa(slots + uniform(step % C::SLOTS) * C::OP), 16, D * 16);
                 if (elect()) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 __syncwarp();
             };
             auto values = [&](int t, int step, bool first) {
-                const uint64_t dv = tc::sdesc_sw128(sa(ring + uniform(step % C::SLOTS) * C::OP), 1024, D * 16);
+                const uint64_t dv = tc::sdesc_sw128(sa(slots + uniform(step % C::SLOTS) * C::OP), 1024, D * 16);
                 // P comes in two halves of 64 positions, each with its barrier (the second may come before the first is seen)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     const int r0 = max(w.kv - p0, 0);
                     for (int e = i; e < (kLongUnit - r0) * (D / 8); e += 128) {
                         const int r = r0 + e / (D / 8), ch = e % (D / 8);
-                        *reinterpret_cast<uint4 *>(ring + s * C::OP + kv_offset<D>(r, ch)) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(slots + s * C::OP + kv_offset<D>(r, ch)) = make_uint4(0, 0, 0, 0);
                     }
                     tc::fence_proxy_async();
                     __syncwarp();
