@@ -172,23 +172,24 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         return max(0, min(w.n, u - w.p.unit));
     };
 
-    Ring ring{full, empty, C::OP, abort_flag, a.err};
-    if (warp == 0) {  // loads
+    if (warp == 0) {  // loads: a ring of K and V in turn, and one of a single stage for the item's rows of q
+        Ring ring{full, empty, C::OP, abort_flag, a.err}, q_ring{qfull, qempty, 0, abort_flag, a.err};
         const int rows = min(a.page_size, kBoxRows), pages = kLongUnit / rows;  // a box each
         int it = 0, item = 0;
         bool ok = true;
         do {
             if (lane == 0) {
-                ok = mbar_wait(qempty, (item & 1) ^ 1, abort_flag, a.err);
+                const int first = w.p.tile * 2 * tq, tiles = first + tq < w.q ? 2 : 1;
+                q_ring.bytes = tiles * (D / 64) * tq * group * 128;
+                ok = ring_claim(q_ring, 1, item);
                 if (ok) {
-                    const int first = w.p.tile * 2 * tq, tiles = first + tq < w.q ? 2 : 1;
-                    mbar_expect_tx(qfull, tiles * (D / 64) * tq * group * 128);
                     for (int t = 0; t < tiles; ++t)
                         for (int h = 0; h < D / 64; ++h)
                             tma_load_4d(sq + t * C::OP + h * C::HALF, &maps.q, h * 64, 0, w.p.head, w.q0 + first + t * tq, qfull);
                 }
             }
             ok = __shfl_sync(~0u, ok, 0);
+            item += ok;
             for (int u = 0; ok && u < w.n; ++u) {
                 const int pos = (w.p.unit + u) * kLongUnit + lane * rows;
                 int place = maps.kv.outside;
@@ -197,20 +198,18 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     if (e >= 0 && e < a.n_pages) place = e * maps.kv.page_step + w.p.head * maps.kv.head_step;
                     else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
                 }
-                for (int kv = 0; ok && kv < 2; ++kv, ++it) {
+                for (int kv = 0; kv < 2; ++kv, ++it) {
                     const int s = it % C::SLOTS;
-                    if (lane == 0) {
-                        ok = mbar_wait(&empty[s], ((it / C::SLOTS) & 1) ^ 1, abort_flag, a.err);
-                        if (ok) mbar_expect_tx(&full[s], C::OP);
-                    }
+                    if (lane == 0) ok = ring_claim(ring, C::SLOTS, it);
                     ok = __shfl_sync(~0u, ok, 0);
-                    if (ok && lane < pages)
+                    if (!ok) break;
+                    if (lane < pages)
                         tma_load_5d(slots + s * C::OP + lane * rows * D * 2, kv ? &maps.kv.v : &maps.kv.k, pos % a.page_size / 8, place, &full[s]);
                 }
             }
-            ++item;
         } while (ok && w.next(a));
-        if (!ok) ring_drain(ring, C::SLOTS, it);
+        ring_drain(q_ring, 1, item);
+        ring_drain(ring, C::SLOTS, it);
     } else if (warp == 1) {  // products, tile 0 and tile 1 in turn
         // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers. From inside a
         // one-lane branch a product took about 110 cycles to issue, against 64 to run.

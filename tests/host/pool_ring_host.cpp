@@ -101,7 +101,7 @@ struct Barrier {  // counts arrivals and bytes; a phase ends when neither is mis
     }
 };
 
-constexpr int STAGES = 3, USERS = 4, BYTES = 100;
+constexpr int STAGES = 6, USERS = 4, BYTES = 100;
 
 struct Block {
     Barrier full[STAGES], empty[STAGES];
@@ -140,9 +140,9 @@ struct Thread {  // the barriers as one thread sees them; `fail`: one wait of so
     }
 };
 
-static void block(unsigned seed, int loads, int fail) {
+static void block(unsigned seed, int stages, int loads, int fail) {
     Block k;
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < stages; ++i) {
         k.full[i].init(1);
         k.empty[i].init(USERS);
     }
@@ -163,9 +163,9 @@ static void block(unsigned seed, int loads, int fail) {
                 std::this_thread::yield();
                 continue;
             }
-            k.stage[it % STAGES] = it;
+            k.stage[it % stages] = it;
             --k.left;
-            k.full[it % STAGES].arrived(BYTES);
+            k.full[it % stages].arrived(BYTES);
         }
     });
     std::vector<std::thread> threads;
@@ -173,13 +173,13 @@ static void block(unsigned seed, int loads, int fail) {
         Thread b{k, seed * 31u + 5, fail, 0};
         int it = 0;
         for (; it < loads; ++it) {
-            if (!ring_claim(b, STAGES, it)) break;
+            if (!ring_claim(b, stages, it)) break;
             ++k.left;
             std::lock_guard<std::mutex> lk(k.mu);
             k.under_way.push_back(it);
         }
         CHECK(fail || it == loads);
-        ring_drain(b, STAGES, it);
+        ring_drain(b, stages, it);
         CHECK(k.left == 0);
         k.gone = 1;
     });
@@ -190,13 +190,13 @@ static void block(unsigned seed, int loads, int fail) {
                 Thread b{k, seed * 131u + w * 17 + l + 3, fail, w};
                 bool alive = true;
                 for (int it = 0; it < loads; ++it) {
-                    alive = ring_take(b, STAGES, it, alive);
-                    if (alive) CHECK(k.stage[it % STAGES] == it);
+                    alive = ring_take(b, stages, it, alive);
+                    if (alive) CHECK(k.stage[it % stages] == it);
                     saw[w][l] = alive;
                     b.all(true);  // (the lanes have used the stage)
                     if (l == 0) {
                         CHECK(saw[w][0] == saw[w][1]);
-                        ring_free(b, STAGES, it, alive);
+                        ring_free(b, stages, it, alive);
                     }
                     b.all(true);
                 }
@@ -208,7 +208,7 @@ static void block(unsigned seed, int loads, int fail) {
 
 int main() {
     for (unsigned i = 1; i <= 300 && !bad; ++i) lanes_agree(i);
-    for (unsigned i = 1; i <= 1500 && !bad; ++i) block(i, 1 + i % 23, i % 5 == 0 ? 0 : i % 3 == 0 ? 2 : 12);
+    for (unsigned i = 1; i <= 1500 && !bad; ++i) block(i, i % 7 == 0 ? 1 : i % 2 ? 3 : 4 + i % 3, 1 + i % 23, i % 5 == 0 ? 0 : i % 3 == 0 ? 2 : 12);
     if (!bad) std::printf("ok\n");
     return bad != 0;
 }
