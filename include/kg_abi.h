@@ -592,6 +592,11 @@ int kg_set_mlp_hook(kg_ctx *ctx, float keep, uint64_t seed);
  * Returns KG_ERR_TIMEOUT (the status a lost arrival inside a GEMM or
  * attention kernel produces); the context stays usable afterwards. */
 int kg_selftest_wait_timeout(kg_ctx *ctx, int64_t limit_cycles);
+/* The same for the kernels of kg_pool_attend_dev: the waits of this context's
+ * later calls run out after limit_cycles SM clocks (at most 2^30; 0: the usual
+ * limit again). A call whose waits run out leaves its rows of out undefined and
+ * KG_ERR_TIMEOUT for kg_pool_status; later calls are not affected. */
+int kg_selftest_pool_wait(kg_ctx *ctx, int64_t limit_cycles);
 /* Kernel launches replayed by the last kg_forward_batch(_dev) call when it ran
  * as a captured CUDA graph (single-position decode of the bf16 path on a
  * non-legacy stream, profiling off); 0 when that call ran eagerly. */

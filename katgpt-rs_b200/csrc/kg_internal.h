@@ -165,6 +165,7 @@ struct kg_ctx {
     float *rot = nullptr, *rot_t = nullptr, *kc = nullptr, *kb = nullptr, *vc = nullptr, *vb = nullptr;
     int *d_err = nullptr;
     int *serve_err = nullptr;  // device-side checks of the kg_pool calls, read by kg_pool_status
+    int serve_quick = 0;  // a test's limit for their device-side waits (clock cycles), 0 for the usual one
     // host copies of the TurboQuant tables
     std::vector<float> h_rot, h_kc, h_kb, h_vc, h_vb, h_pred;
     // decode step graphs (bf16 path, T == 1): inputs are copied into the

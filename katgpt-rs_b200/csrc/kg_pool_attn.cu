@@ -76,7 +76,7 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
 }
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <typename T, int D>
+template <typename T, int D, bool QUICK>
 __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __grid_constant__ PoolMap maps, const AttendArgs a,
                                                                    int after_long) {
     using C = ShortCfg<D>;
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
     Walk<false> w;
     w.start(a, req, off, units);
 
-    Ring ring{full, empty, 2 * C::OP_BYTES, abort_flag, a.err};
+    Ring<QUICK> ring{full, empty, 2 * C::OP_BYTES, abort_flag, a};
     if (warp == 4) {  // producer: lane i loads box i of a unit
         const int rows = min(a.page_size, kBoxRows), pages = C::UNIT / rows, boxes = pages * 2;
         const int piece = lane % pages, which = lane / pages;
@@ -462,7 +462,7 @@ Space space_of(const kg_pool &p, int n_head, int total_q) {
     return s;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool QUICK>
 cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *workspace, cudaStream_t s) {
     PoolMap maps;
     std::memset(&maps, 0, sizeof(maps));
@@ -474,11 +474,11 @@ cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *worksp
     int parts = held[device].load(std::memory_order_acquire);
     cudaError_t e = cudaSuccess;
     if (parts == 0) {
-        e = dev::smem(attend_short_kernel<T, D>, C::SMEM);
-        if (e == cudaSuccess) e = dev::whole_smem(attend_short_kernel<T, D>);
+        e = dev::smem(attend_short_kernel<T, D, QUICK>, C::SMEM);
+        if (e == cudaSuccess) e = dev::whole_smem(attend_short_kernel<T, D, QUICK>);
         if (e == cudaSuccess) e = dev::whole_smem(attend_join_kernel<T, D>);
         if (e != cudaSuccess) return e;
-        parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D>, SHORT_THREADS, C::SMEM));
+        parts = std::min(kMaxParts, dev::sm_count() * dev::occupancy(attend_short_kernel<T, D, QUICK>, SHORT_THREADS, C::SMEM));
         held[device].store(parts, std::memory_order_release);
     }
     AttendArgs b = a;
@@ -496,9 +496,14 @@ cudaError_t launch(const kg_pool &p, const Space &sp, AttendArgs a, void *worksp
     a.part = reinterpret_cast<float *>(a.meta + 2 * kMaxParts);
     a.slot_floats = sp.slot_floats;
     a.rows = sp.rows;
-    e = launch_pdl(attend_short_kernel<T, D>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a, (int)sp.may_long);
+    e = launch_pdl(attend_short_kernel<T, D, QUICK>, dim3(parts), dim3(SHORT_THREADS), C::SMEM, s, maps, a, (int)sp.may_long);
     if (e != cudaSuccess) return e;
     return launch_pdl(attend_join_kernel<T, D>, dim3(parts * JOIN_SHORT + long_parts * JOIN_LONG), dim3(256), 0, s, a, parts, b);
+}
+template <bool QUICK>
+cudaError_t launch(const kg_pool &p, const Space &sp, const AttendArgs &a, void *ws, cudaStream_t s) {
+    if (p.dtype == KG_DT_BF16) return p.head_dim == 64 ? launch<__nv_bfloat16, 64, QUICK>(p, sp, a, ws, s) : launch<__nv_bfloat16, 128, QUICK>(p, sp, a, ws, s);
+    return p.head_dim == 64 ? launch<__half, 64, QUICK>(p, sp, a, ws, s) : launch<__half, 128, QUICK>(p, sp, a, ws, s);
 }
 
 int check(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t n_head, int32_t total_q) {
@@ -568,10 +573,9 @@ int kg_pool_attend_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_req, int32_t 
     a.o_head = out_head_stride;
     a.scale = std::max(scale * 1.4426950408889634f, FLT_MIN);  // (a masked score, -inf, times 0 would be NaN)
     a.err = ctx->serve_err;
+    a.quick = ctx->serve_quick;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool bf = pool->dtype == KG_DT_BF16;
-    const cudaError_t e = pool->head_dim == 64 ? (bf ? launch<__nv_bfloat16, 64>(*pool, sp, a, workspace, s) : launch<__half, 64>(*pool, sp, a, workspace, s))
-                                               : (bf ? launch<__nv_bfloat16, 128>(*pool, sp, a, workspace, s) : launch<__half, 128>(*pool, sp, a, workspace, s));
+    const cudaError_t e = a.quick ? launch<true>(*pool, sp, a, workspace, s) : launch<false>(*pool, sp, a, workspace, s);
     return e == cudaSuccess ? KG_OK : cuda_fail(ctx, e, "kg_pool_attend_dev");
 }
 

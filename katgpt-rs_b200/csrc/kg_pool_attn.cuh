@@ -25,6 +25,7 @@ struct AttendArgs {
     int64_t q_row, q_head, o_row, o_head;
     float scale;  // times log2(e)
     int *err;
+    int quick;  // clock cycles of the QUICK kernels' waits; 0: the usual kernels
     // partial results: slot 2 c of CTA c for the item its part begins inside, slot 2 c + 1 for the one it
     // ends inside without having begun in; `rows` rows of head_dim sums, then rows of (max, sum)
     float *part;
@@ -72,24 +73,43 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// The kernels are built twice: QUICK ones, for a test, whose waits run out after a.quick clock cycles (mbarrier.try_wait may
+// sleep for longer, test_wait does not). Choosing at run time cost the long requests' kernel 6%.
+template <bool QUICK>
+__device__ __forceinline__ bool bounded_wait(uint64_t *bar, int parity, volatile int *abort_flag, const AttendArgs &a) {
+    if (!QUICK) return as::mbar_wait(bar, parity, abort_flag, a.err);
+    const long long t0 = clock64();
+    do {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok)
+                     : "r"(as::sa(bar)), "r"(parity)
+                     : "memory");
+        if (ok) return true;
+    } while (!*abort_flag && clock64() - t0 < a.quick);
+    *abort_flag = 1;
+    atomicExch(a.err, (int)KG_ERR_TIMEOUT);
+    return false;
+}
+// for what ends whatever else happened (bounded all the same)
+__device__ __forceinline__ void wait_done(uint64_t *bar, int parity) {
+    const long long t0 = clock64();
+    while (!as::mbar_try(bar, parity) && clock64() - t0 < (1ll << 28)) {
+    }
+}
 // The barriers of a ring of stages (kg_pool_ring.h), `bytes` in each.
+template <bool QUICK>
 struct Ring {
     uint64_t *full, *empty;
     uint32_t bytes;
     volatile int *abort_flag;
-    int *err;
-    __device__ __forceinline__ bool wait_full(int s, int parity) { return as::mbar_wait(&full[s], parity, abort_flag, err); }
-    __device__ __forceinline__ bool wait_empty(int s, int parity) { return as::mbar_wait(&empty[s], parity, abort_flag, err); }
+    const AttendArgs &a;
+    __device__ __forceinline__ bool wait_full(int s, int parity) { return bounded_wait<QUICK>(&full[s], parity, abort_flag, a); }
+    __device__ __forceinline__ bool wait_empty(int s, int parity) { return bounded_wait<QUICK>(&empty[s], parity, abort_flag, a); }
     __device__ __forceinline__ void arm(int s) { as::mbar_expect_tx(&full[s], bytes); }
     __device__ __forceinline__ void free(int s) { as::mbar_arrive(&empty[s]); }
     __device__ __forceinline__ bool all(bool x) { return __all_sync(~0u, x) != 0; }
-    // a load that has been issued ends whatever else happened (bounded all the same)
-    __device__ __forceinline__ void landed(int s, int parity) { wait_landed(&full[s], parity); }
-    static __device__ __forceinline__ void wait_landed(uint64_t *bar, int parity) {
-        const long long t0 = clock64();
-        while (!as::mbar_try(bar, parity) && clock64() - t0 < (1ll << 28)) {
-        }
-    }
+    __device__ __forceinline__ void landed(int s, int parity) { wait_done(&full[s], parity); }
 };
 
 // Shared-memory form of K and V: groups of 8 positions, each [head_dim / 64][8

@@ -47,7 +47,7 @@ struct LongCfg {
     static constexpr int HALF = 128 * 128;           // 128 rows x 64 elements
     static constexpr int OP = HALF * (D / 64);       // a Q tile, or K or V of a unit
     static constexpr int SLOTS = D == 64 ? 6 : 4;    // K and V in turn
-    static constexpr int BARS = 2 * SLOTS + 2 + 8;
+    static constexpr int BARS = 2 * SLOTS + 2 + 8 + 1;
     static constexpr int SMEM = 1024 + 2 * OP + SLOTS * OP + BARS * 8 + 16;
 };
 
@@ -115,7 +115,7 @@ struct LongMaps {
     PoolMap kv;
 };
 
-template <typename T, int D>
+template <typename T, int D, bool QUICK>
 __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __grid_constant__ LongMaps maps, const AttendArgs a) {
     using C = LongCfg<D>;
     extern __shared__ __align__(1024) uint8_t raw[];
@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     uint64_t *full = reinterpret_cast<uint64_t *>(slots + C::SLOTS * C::OP), *empty = full + C::SLOTS;
     uint64_t *qfull = empty + C::SLOTS, *qempty = qfull + 1;
     uint64_t *sfull = qempty + 1, *pvdone = sfull + 2, *pready = pvdone + 2;  // [2] by tile, pready [tile][half]
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(pready + 4);
+    uint64_t *last = pready + 4;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(last + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tslot + 1);
     __shared__ long long part_sm[2 * (LONG_THREADS / 32) + 2];
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, c = blockIdx.x;
@@ -136,6 +137,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
         }
         mbar_init(qfull, 1);
         mbar_init(qempty, 1);
+        mbar_init(last, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sfull[t], 1);
             mbar_init(&pready[2 * t], 4);
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
     };
 
     if (warp == 0) {  // loads: a ring of K and V in turn, and one of a single stage for the item's rows of q
-        Ring ring{full, empty, C::OP, abort_flag, a.err}, q_ring{qfull, qempty, 0, abort_flag, a.err};
+        Ring<QUICK> ring{full, empty, C::OP, abort_flag, a}, q_ring{qfull, qempty, 0, abort_flag, a};
         const int rows = min(a.page_size, kBoxRows), pages = kLongUnit / rows;  // a box each
         int it = 0, item = 0;
         bool ok = true;
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             constexpr uint32_t IDS = tc::idesc_f16(FMT, 128, 128), IDO = tc::idesc_f16(FMT, 128, D, 0, 1);
             int it = 0, item = 0, cnt[2] = {0, 0};
             bool ok = true;
-            auto wait = [&](uint64_t *b, int parity) { return __all_sync(~0u, mbar_wait(b, parity, abort_flag, a.err)) != 0; };
+            auto wait = [&](uint64_t *b, int parity) { return __all_sync(~0u, bounded_wait<QUICK>(b, parity, abort_flag, a)) != 0; };
             auto wait_slot = [&](int step) { return wait(&full[step % C::SLOTS], (step / C::SLOTS) & 1); };
             auto scores = [&](int t, int step) {
                 const uint64_t dq = tc::sdesc_k(sq + t * C::OP), dk = tc::sdesc_sw128(sa(slots + uniform(step % C::SLOTS) * C::OP), 16, D * 16);
@@ -291,6 +293,11 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 }
                 ++item;
             } while (ok && w.next(a));
+            // Whoever's wait ran out: the products issued so far are done before their tensor memory and shared memory are
+            // given back.
+            if (elect()) tc::commit(last);
+            __syncwarp();
+            wait_done(last, 0);
         }
     } else {  // rows of tile t: warp's lanes are tensor-memory lanes 32 (warp % 4) ..
         const int t = warp >= 6, q4 = warp & 3, i = q4 * 32 + lane;
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             const int n = n_of(t);
             float m = -INFINITY, l = 0.0f;
             for (int u = 0; ok && u < n; ++u, ++cnt) {
-                ok = mbar_wait(&sfull[t], cnt & 1, abort_flag, a.err);
+                ok = bounded_wait<QUICK>(&sfull[t], cnt & 1, abort_flag, a);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 tc::fence_after();
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                     const float next = base_of(top, Cvt<T>::UP_LONG), f = up ? exp2_approx(m - next) : 1.0f;
                     if (up) m = next;
                     l *= f;
-                    ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
+                    ok = __all_sync(~0u, bounded_wait<QUICK>(&pvdone[t], (cnt - 1) & 1, abort_flag, a));
                     if (!ok) break;
                     tc::fence_after();
 #pragma unroll 1
@@ -360,7 +367,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 }
                 if (p0 + kLongUnit > w.kv) {  // V rows behind the last position: whatever the page holds must not reach the sums
                     const int it = v_it + 2 * u, s = it % C::SLOTS;
-                    ok = __all_sync(~0u, mbar_wait(&full[s], (it / C::SLOTS) & 1, abort_flag, a.err));
+                    ok = __all_sync(~0u, bounded_wait<QUICK>(&full[s], (it / C::SLOTS) & 1, abort_flag, a));
                     if (!ok) break;
                     const int r0 = max(w.kv - p0, 0);
                     for (int e = i; e < (kLongUnit - r0) * (D / 8); e += 128) {
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 l += s0 + s1;
             }
             // the item's rows
-            if (ok && n > 0) ok = __all_sync(~0u, mbar_wait(&pvdone[t], (cnt - 1) & 1, abort_flag, a.err));
+            if (ok && n > 0) ok = __all_sync(~0u, bounded_wait<QUICK>(&pvdone[t], (cnt - 1) & 1, abort_flag, a));
             if (!ok) break;
             tc::fence_after();
             const bool whole = w.whole();
@@ -436,6 +443,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
             }
             v_it += 2 * w.n;
         } while (w.next(a));
+        tc::st_wait();
     }
     tc::fence_before();
     __syncthreads();
@@ -460,7 +468,7 @@ bool q_map(CUtensorMap *m, const AttendArgs &a, int d) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool QUICK>
 cudaError_t launch(const PoolMap &kv, const AttendArgs &a, int parts, cudaStream_t s) {
     LongMaps maps;
     std::memset(&maps, 0, sizeof(maps));
@@ -470,12 +478,17 @@ cudaError_t launch(const PoolMap &kv, const AttendArgs &a, int parts, cudaStream
     static std::atomic<bool> set[64];  // attributes, per device
     const int device = dev::current() & 63;
     if (!set[device].load(std::memory_order_acquire)) {
-        cudaError_t e = dev::smem(attend_long_kernel<T, D>, C::SMEM);
-        if (e == cudaSuccess) e = dev::whole_smem(attend_long_kernel<T, D>);
+        cudaError_t e = dev::smem(attend_long_kernel<T, D, QUICK>, C::SMEM);
+        if (e == cudaSuccess) e = dev::whole_smem(attend_long_kernel<T, D, QUICK>);
         if (e != cudaSuccess) return e;
         set[device].store(true, std::memory_order_release);
     }
-    return launch_pdl(attend_long_kernel<T, D>, dim3(parts), dim3(LONG_THREADS), C::SMEM, s, maps, a);
+    return launch_pdl(attend_long_kernel<T, D, QUICK>, dim3(parts), dim3(LONG_THREADS), C::SMEM, s, maps, a);
+}
+
+template <typename T, int D>
+cudaError_t launch(const PoolMap &kv, const AttendArgs &a, int parts, cudaStream_t s) {
+    return a.quick ? launch<T, D, true>(kv, a, parts, s) : launch<T, D, false>(kv, a, parts, s);
 }
 
 }  // namespace

@@ -6,7 +6,8 @@
 // KG_ERR_TIMEOUT to the context's error word and returns, so a lost arrival
 // ends the call with an error status and the context stays usable. This
 // kernel exercises exactly that path on purpose with a short limit: one
-// thread waits on a barrier that nothing arrives on.
+// thread waits on a barrier that nothing arrives on. kg_selftest_pool_wait gives
+// the attention over a page pool a limit so short that its own waits run out.
 #include <cuda_runtime.h>
 
 #include <string>
@@ -51,4 +52,10 @@ extern "C" int kg_selftest_wait_timeout(kg_ctx *ctx, int64_t limit_cycles) {
         return KG_ERR_TIMEOUT;
     }
     return herr ? KG_ERR_CUDA : KG_OK;
+}
+
+extern "C" int kg_selftest_pool_wait(kg_ctx *ctx, int64_t limit_cycles) {
+    if (!ctx || limit_cycles < 0 || limit_cycles > (1 << 30)) return KG_ERR_INVALID_ARG;
+    ctx->serve_quick = (int)limit_cycles;
+    return KG_OK;
 }
