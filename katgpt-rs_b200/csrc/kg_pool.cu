@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(256) store_kernel(StoreArgs a) {
     const int slot = a.slots[row];
     if (slot < 0) return;
     if (slot >= a.places) {
-        if (c == 0 && blockIdx.y == 0) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+        if (c == 0 && blockIdx.y == 0) reject(a.err);
         return;
     }
     const S *src = static_cast<const S *>(blockIdx.y ? a.v : a.k) + row * a.row_stride + h * a.head_stride + d;

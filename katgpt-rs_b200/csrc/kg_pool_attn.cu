@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                 if (lane < boxes && pos < w.kv) {
                     const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
                     if (e >= 0 && e < a.n_pages) place = e * maps.page_step + w.p.head * maps.head_step;
-                    else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+                    else reject(a.err);
                 }
                 if (lane == 0) ok = ring_claim(ring, C::STAGES, it);
                 ok = __shfl_sync(~0u, ok, 0);

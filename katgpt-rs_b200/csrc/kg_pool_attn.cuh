@@ -9,6 +9,7 @@
 
 #include "kg_async.cuh"
 #include "kg_pool_ring.h"
+#include "kg_serve.h"
 
 namespace kg {
 namespace serve {
@@ -168,7 +169,7 @@ __device__ void find_part(const AttendArgs &a, int c, int parts, int least, long
     long long mine = 0, items = 0;
     for (int r = r0; r < r1; ++r) {
         int q0, q, kv;
-        if (!req_len(a, r, q0, q, kv) && c == 0) atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+        if (!req_len(a, r, q0, q, kv) && c == 0) reject(a.err);
         mine += request_units(a.s, LONG, q, kv);
         items += request_items(a.s, LONG, q, kv);
     }

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 if (lane < pages && pos < w.kv) {
                     const int e = a.table[(int64_t)w.r * a.width + pos / a.page_size];
                     if (e >= 0 && e < a.n_pages) place = e * maps.kv.page_step + w.p.head * maps.kv.head_step;
-                    else atomicExch(a.err, (int)KG_ERR_INVALID_ARG);
+                    else reject(a.err);
                 }
                 for (int kv = 0; kv < 2; ++kv, ++it) {
                     const int s = it % C::SLOTS;

@@ -16,6 +16,13 @@ namespace serve {
 constexpr int kMaxReq = 16384;     // requests of one call
 constexpr int kMaxVocab = 262144;  // 2^18 weights of at most 2^44 sum below 2^63
 
+#ifdef __CUDACC__
+// An argument that a device-side check turned down, for kg_pool_status. KG_ERR_TIMEOUT, the lower number, stays: it is
+// about every row of a call, not about the ones that were named.
+__device__ __forceinline__ void reject(int *err) { atomicMin(err, (int)KG_ERR_INVALID_ARG); }
+static_assert(KG_ERR_TIMEOUT < KG_ERR_INVALID_ARG && KG_ERR_INVALID_ARG < KG_OK, "the lowest status stays");
+#endif
+
 // Message of the calling thread's last call without a context.
 std::string &thread_error();
 inline int fail(kg_ctx *ctx, int code, const std::string &msg) {

@@ -74,3 +74,41 @@ def test_waits_that_run_out_end_the_call(kg, case):
         assert torch.equal(call.out, want)
     assert ran_out > 0
     be.close()
+
+
+def test_a_rejected_argument_does_not_hide_a_wait_that_ran_out(kg):
+    import torch
+    be = kg.CudaBackend(kg.micro_config())
+    lib = kg.lib()
+    call = Call(kg, be, *CASES[4])
+    rows = torch.zeros(1, 1, call.d, device="cuda")
+    slot = torch.full((1,), 1 << 20, dtype=torch.int32, device="cuda")  # past the pool
+    cu = call.cu.clone()
+
+    def reject_store():
+        be.pool_store_dev(call.pool, 1, slot.data_ptr(), "f32", rows.data_ptr(), rows.data_ptr(), call.d, call.d)
+
+    def reject_lengths():
+        call.cu.copy_(cu + call.total)
+        call()
+        call.cu.copy_(cu)
+
+    def reject_table(reqs):
+        keep = call.table.clone()
+        call.table[reqs, 0] = -5
+        call()
+        call.table.copy_(keep)
+
+    for reject in (reject_store, reject_lengths, lambda: reject_table(1), lambda: reject_table(0)):
+        lib.kg_selftest_pool_wait(be._h, 1)
+        call()
+        lib.kg_selftest_pool_wait(be._h, 0)
+        reject()
+        with pytest.raises(kg.KgError, match="exceeded") as e:
+            be.pool_status()
+        assert e.value.status == -4
+        reject()
+        with pytest.raises(kg.KgError, match="rejected"):
+            be.pool_status()
+        be.pool_status()
+    be.close()
