@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs a) {
     if (code != KG_OK) {  // the step does nothing
         for (int r = gid; r <= a.n_req; r += step) a.cu[r] = 0;
         for (int r = gid; r < a.n_req; r += step) a.kv[r] = 0;
-        for (int i = gid; i < a.max_tokens; i += step) a.slots[i] = a.req[i] = a.pos[i] = -1;
+        for (uint32_t i = gid; i < (uint32_t)a.max_tokens; i += step) a.slots[i] = a.req[i] = a.pos[i] = -1;
     } else {
         for (int r = gid; r <= a.n_req; r += step) a.cu[r] = cu[r];
         for (int r = gid; r < a.n_req; r += step) a.kv[r] = old[r] + cu[r + 1] - cu[r];
@@ -170,12 +170,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs a) {
             a.table[(int64_t)r * a.width + pages_of(old[r], shift) + i - pg[r]] = a.free_pages[nf - 1 - i];
         }
 #pragma unroll 4
-        for (int i = gid; i < a.max_tokens; i += step) {
+        for (uint32_t i = gid; i < (uint32_t)a.max_tokens; i += step) {  // (i may pass 2^31 by a step)
             int slot = -1, r = -1, x = -1;
-            if (i < (int)tokens) {
-                r = range_of(cu, a.n_req, i);
+            if (i < (uint32_t)tokens) {
+                r = range_of(cu, a.n_req, (int)i);
                 const int c = old[r];
-                x = c + i - cu[r];
+                x = c + (int)i - cu[r];
                 const int has = pages_of(c, shift), q = x >> shift;
                 const int e = __ldg(q < has ? a.table + (int64_t)r * a.width + q : a.free_pages + (nf - 1 - (pg[r] + q - has)));
                 slot = (e << shift) + (x & (a.page - 1));

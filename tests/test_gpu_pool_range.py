@@ -86,3 +86,24 @@ def test_scores_past_the_whole_numbers_of_f32(kg, be, dt, rows, sign):
             k[..., 0] = sign * f * 2.0 ** e
             got, want, tol = _shared(kg, be, k, v, q, 1, dt, 1.0, 0)
             assert (np.abs(got - want) <= tol).all(), (e, f)
+
+
+@pytest.mark.parametrize("fits", [True, False])
+def test_a_plan_with_room_for_two_billion_tokens(be, fits):
+    """The largest max_tokens (26 GB of token entries): the padding ends where the entries do."""
+    import torch
+    m = 2**31 - 1
+    i32 = dict(dtype=torch.int32, device="cuda")
+    slots, req, pos = (torch.full((m + 9,), 777, **i32) for _ in range(3))
+    cached, new, table = torch.tensor([5, 0], **i32), torch.tensor([3, 20 if fits else -1], **i32), torch.zeros(2, 4, **i32)
+    free, n_free, left = torch.arange(1, 8, **i32), torch.tensor([7], **i32), torch.zeros(1, **i32)
+    cu, kv, status = torch.zeros(3, **i32), torch.zeros(2, **i32), torch.zeros(1, **i32)
+    p = lambda x: x.data_ptr()  # noqa: E731
+    be.pool_plan_dev(16, 8, 2, p(cached), p(new), p(table), 4, p(free), p(n_free), p(left), m, p(cu), p(kv), p(slots), p(req), p(pos), p(status))
+    torch.cuda.synchronize()
+    total = 23 if fits else 0
+    assert int(status) == (0 if fits else -1) and cu.tolist() == ([0, 3, 23] if fits else [0, 0, 0])
+    for x in (slots, req, pos):
+        assert (x[:total] >= 0).all() and (x[m:] == 777).all()
+        for at in range(total, m, 1 << 28):
+            assert (x[at:min(at + (1 << 28), m)] == -1).all()
