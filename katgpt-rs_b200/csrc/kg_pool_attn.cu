@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attend_short_kernel(const __gri
                 float total = 0.0f;
                 for (int k = g; k < 4; k += wm) {
                     const float2 x = stat[k * 16 + r];
-                    if (x.x != -INFINITY) total += x.y * exp2_approx(x.x - top);
+                    total += x.x == -INFINITY ? x.y : x.y * exp2_approx(x.x - top);  // (there a sum is 0, or NaN as its scores)
                 }
                 if (whole) {
                     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendArgs sh, i
 #pragma unroll 4
         for (int k = first; k < n; k += step) {
             const float2 s = stat_of(k);
-            if (s.x == -INFINITY) continue;  // nothing was attended there, nothing was written
+            if (s.x == -INFINITY && s.y == 0.0f) continue;  // nothing was attended there (a sum that is NaN is to be seen)
             const float f = exp2_approx(s.x - top);
             const float *p = slot(k) + (int64_t)row * D + lane * PER;
             l += s.y * f;

@@ -107,3 +107,45 @@ def test_a_plan_with_room_for_two_billion_tokens(be, fits):
         assert (x[:total] >= 0).all() and (x[m:] == 777).all()
         for at in range(total, m, 1 << 28):
             assert (x[at:min(at + (1 << 28), m)] == -1).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("reqs,n_head,n_kv,d", [
+    ([(2, 9000), (3, 2), (1, 40)], 4, 2, 128),   # short: positions split over the device, whole, rows before position 0
+    ([(1, 900)] * 400, 2, 2, 64),
+    ([(100, 9000), (70, 30), (80, 80)], 4, 2, 128),  # long
+    ([(90, 300)] * 60, 2, 1, 64),
+])
+def test_a_query_that_is_not_a_number(kg, be, bad, reqs, n_head, n_kv, d):
+    """Its rows come out as NaN wherever the items are cut, a row that attends nothing as zeros, the others as they are."""
+    import torch
+    page, pages = 16, 600
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m = torch.randn(pages, 2, page, n_kv, d, generator=g, device="cuda").half()
+    pool = kg.page_pool(m.data_ptr(), m[0, 1].data_ptr(), pages, page, n_kv, d, "f16")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q_len, kv = [r[0] for r in reqs], [r[1] for r in reqs]
+    cu, kvd = torch.tensor([0] + list(np.cumsum(q_len)), **i32), torch.tensor(kv, **i32)
+    table = torch.arange(pages, **i32).repeat(len(reqs), 1)
+    total = sum(q_len)
+    q = torch.randn(total, n_head, d, generator=g, device="cuda").half()
+    ws = torch.full((be.pool_attend_bytes(pool, len(reqs), n_head, total),), 0xFF, dtype=torch.uint8, device="cuda")
+
+    def run(q):
+        out = torch.full_like(q, 7.0)
+        be.pool_attend_dev(pool, len(reqs), n_head, total, cu.data_ptr(), kvd.data_ptr(), table.data_ptr(), pages, q.data_ptr(), q.stride(0),
+                           q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), d ** -0.5, 1, ws.data_ptr(), ws.numel())
+        torch.cuda.synchronize()
+        be.pool_status()
+        return out
+    good = run(q)
+    hit = torch.zeros(total, n_head, dtype=torch.bool, device="cuda")
+    hit[::3, n_head - 1] = True
+    hit[1::5, 0] = True
+    hit[cu[:-1].long()] = True
+    none = torch.cat([torch.arange(a, device="cuda") - a + b < 0 for a, b in reqs])[:, None].expand_as(hit)  # attends nothing
+    q2 = q.clone()
+    q2[..., 3] = torch.where(hit, torch.full_like(q2[..., 3], bad), q2[..., 3])
+    got = run(q2)
+    assert (got[hit & ~none].isnan()).all()
+    assert (got[none] == 0).all() and torch.equal(got[~hit], good[~hit])
