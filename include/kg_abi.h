@@ -318,7 +318,7 @@ int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const in
  * page_size] and below 2^31 - 256, or the request's rows are left as they were; a
  * table entry outside the pool reads as zeros; either is reported. n_head at most
  * 64 times n_kv_head, at most 16384 requests.
- * workspace: kg_pool_attend_bytes() bytes (77 MB at most), 16-byte aligned, for
+ * workspace: kg_pool_attend_bytes() bytes (64 MB at most), 16-byte aligned, for
  * partial results when one request's positions are split over several CTAs; its
  * content need not be kept or initialised, and calls that may overlap on the device
  * (other streams, two graphs) need one each. kg_pool_attend_bytes returns a negative

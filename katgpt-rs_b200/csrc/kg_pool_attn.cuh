@@ -15,7 +15,7 @@ namespace kg {
 namespace serve {
 
 constexpr int kBoxRows = 64;  // page rows of a TMA box at most
-constexpr int kMaxParts = 512, kMaxLongParts = 160;  // CTAs of the two kernels' lines at most (3 and 1 per SM of a B200)
+constexpr int kMaxParts = 320, kMaxLongParts = 160;  // CTAs of the two kernels' lines at most (2 and 1 on each of a B200's 148 SMs)
 
 struct AttendArgs {
     Shape s;
