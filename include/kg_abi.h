@@ -307,17 +307,19 @@ int kg_pool_store_dev(kg_ctx *ctx, const kg_pool *pool, int32_t n_rows, const in
  * does over its prompt). Query head h reads KV head h / (n_head / n_kv_head):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]
  * (scale not negative) with f32 scores, statistics and sums; a row that attends
- * nothing (kv_len 0, or a row before position 0) becomes zeros. The probabilities
- * enter the second product in the pool's type (in f16 those below 2^-26 of a row's
- * largest lose bits, those below 2^-36 are 0), everything is rounded once at the end. The same call gives the same bits; how a request's sums are cut, and with
- * it their last bits, depends on the batch that it is in. q and out have the pool's
- * type, out row i head h at i * out_row_stride + h * out_head_stride; q and out must
- * not overlap. Rows outside every request's range are left as they were. Page
- * contents past kv_len are never used; those before it are finite. Device-side
- * checks: cu_q non-decreasing within [0, total_q], kv_len within [0, table_width *
- * page_size] and below 2^31 - 256, or the request's rows are left as they were; a
- * table entry outside the pool reads as zeros; either is reported. n_head at most
- * 64 times n_kv_head, at most 16384 requests.
+ * nothing (kv_len 0, or a row before position 0) becomes zeros, one with a NaN in q
+ * becomes NaN. The probabilities enter the second product in the pool's type (in f16
+ * those below 2^-26 of a row's largest lose bits, those below 2^-37 are 0), everything
+ * is rounded once at the end. For requests of more than 64 rows (tokens x n_head /
+ * n_kv_head) scores stay below 2^26. The same call gives the same bits; how a
+ * request's sums are cut, and with it their last bits, depends on the batch that it
+ * is in. q and out have the pool's type, out row i head h at i * out_row_stride +
+ * h * out_head_stride; q and out must not overlap. Rows outside every request's range
+ * are left as they were. Page contents past kv_len are never used; those before it
+ * are finite. Device-side checks: cu_q non-decreasing within [0, total_q], kv_len
+ * within [0, table_width * page_size] and below 2^31 - 256, or the request's rows are
+ * left as they were; a table entry outside the pool reads as zeros; either is
+ * reported. n_head at most 64 times n_kv_head, at most 16384 requests.
  * workspace: kg_pool_attend_bytes() bytes (64 MB at most), 16-byte aligned, for
  * partial results when one request's positions are split over several CTAs; its
  * content need not be kept or initialised, and calls that may overlap on the device

@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(LONG_THREADS, 1) attend_long_kernel(const __gr
                 float top = top_of();
                 half(0);
                 top = fmaxf(top, top_of());
-                top = top == -INFINITY ? top : top * a.scale;
+                // (the exponents take the product with the scale whole: in f16 none may come out above the rounded maximum)
+                top = top == -INFINITY ? top : Cvt<T>::UP_LONG > 0.0f ? __fmul_ru(top, a.scale) : top * a.scale;
                 const bool grow = u == 0 || top - m > Cvt<T>::UP_LONG + Cvt<T>::LAG;
                 if (u == 0) {
                     m = base_of(top, Cvt<T>::UP_LONG);

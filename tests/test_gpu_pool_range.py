@@ -149,3 +149,27 @@ def test_a_query_that_is_not_a_number(kg, be, bad, reqs, n_head, n_kv, d):
     got = run(q2)
     assert (got[hit & ~none].isnan()).all()
     assert (got[none] == 0).all() and torch.equal(got[~hit], good[~hit])
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [2, 70])
+def test_large_scores_of_any_bits(kg, be, dt, rows):
+    """Scores whose product with the scale has more bits than f32: one position of each row is far above the others, so that
+    the row is that position's value. Requests of more than 64 rows promise it up to 2^26."""
+    import torch
+    d, positions = 64, 200
+    rng = np.random.default_rng(11)
+    half = torch.finfo({"bf16": torch.bfloat16, "f16": torch.float16}[dt]).eps / 2
+    for e in range(9):
+        for scale in (0.001, 0.3, 1.0, 7.3, 30.0):
+            if rows > 64 and 2.0 ** (7 + e + 15) * scale > 2.0 ** 26:
+                continue
+            k = np.zeros((positions, 1, d))
+            k[:, 0, 0] = rng.uniform(0.1, 0.5, positions) * 2.0 ** (6 + e)
+            k[rng.integers(0, positions), 0, 0] = rng.uniform(1.0, 2.0) * 2.0 ** (6 + e)
+            q = np.zeros((rows, 2, d))
+            q[..., 0] = rng.uniform(0.5, 1.0, (rows, 2)) * 2.0 ** 15
+            v = rng.uniform(0.5, 1.5, (positions, 1, d))
+            got, want, _ = _shared(kg, be, k, v, q, 1, dt, scale, 0)
+            # the one probability is rounded and divided by itself unrounded, then the result: half a step each
+            assert (np.abs(got - want) <= 2 * half * 1.01 * np.abs(want)).all(), (e, scale, np.abs(got - want).max())
