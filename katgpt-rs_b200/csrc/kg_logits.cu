@@ -20,10 +20,16 @@
 //     is where the running sum from what lies above them arrives; the token is drawn by
 //     all CTAs;
 //   - where a step holds more (rows of equal values), by bisection over the whole row.
-// Bound by the latency of a row's steps: 64 rows of 32000 in 44 us, 256 nucleus rows of
-// 131072 in 500 us (33 clusters at a time, about 50 us a row; read alone, 10 us).
-// Weights cost about 14 operations in 64 bits, which run at a half of the 32-bit
-// rate: they are computed once for top-p's histogram and once for what is drawn from.
+// Bound by the latency of a row's steps (64 rows of 32000 in 44 us; 21 us where every
+// token stays) and by the weights: 256 nucleus rows of 131072 in 500 us, 33 clusters at a
+// time in eight rounds (read alone, 10 us). A weight costs about 14 operations in 64 bits,
+// at half the 32-bit rate, and is computed once for top-p's histogram and once for what
+// is drawn from; 64 registers a thread for two CTAs on an SM spill 124 bytes.
+// Sorting up to 4096 entries of a step, against 2048 and the bisection before it, and
+// candidates in the first CTA: 256 x 131072 nucleus rows of normal logits take 8% to 12%
+// longer at a deviation of 0.5 to 4 (bf16, 2: 460 -> 500 us), but 620 us in place of 1500
+// at 0.3, where steps are crowded, and 690 in place of 2360 at 0.2; 64 mixed rows of 32000
+// 57 -> 49 us, 285 -> 79 at 0.05.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -213,20 +219,20 @@ __global__ void __launch_bounds__(THREADS, 2) sample_logits_kernel(SampleArgs a)
         return warp_sum(v);
     };
     auto scan = [&](u64 v) {  // exclusive, over the block's threads
-                u64 x = v;
-    #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const u64 y = __shfl_up_sync(~0u, x, d);
-                    if (lane >= d) x += y;
-                }
-                u64 *to = sh.warp[flip & 1];
-                ++flip;
-                if (lane == 31) to[warp] = x;
-                __syncthreads();
-                u64 before = 0;
-                for (int k = 0; k < warp; ++k) before += to[k];
-                return before + x - v;
-            };
+        u64 x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const u64 y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
+        }
+        u64 *to = sh.warp[flip & 1];
+        ++flip;
+        if (lane == 31) to[warp] = x;
+        __syncthreads();
+        u64 before = 0;
+        for (int k = 0; k < warp; ++k) before += to[k];
+        return before + x - v;
+    };
     int turn = 0;
     // every CTA's values (v, x, y: the same in all its threads, or those of the thread that names them by `mine`): f(rank, v, x, y)
     auto share = [&](bool mine, u64 v, u64 x, u64 y, auto f) {

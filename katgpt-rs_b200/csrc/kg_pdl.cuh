@@ -5,7 +5,9 @@
 // previous one drains. Every kernel launched this way calls pdl_wait() before
 // its first global-memory access: griddepcontrol.wait blocks until the grids
 // it depends on have completed and their memory is visible (a no-op after an
-// ordinary launch or a memory operation).
+// ordinary launch or a memory operation). One kernel waits only before it ends:
+// attend_short_kernel behind attend_long_kernel, whose CTAs have all waited when
+// it starts and whose results it does not touch.
 #pragma once
 #include <cuda_runtime.h>
 

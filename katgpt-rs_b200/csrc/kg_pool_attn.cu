@@ -36,9 +36,10 @@ using namespace as;
 // dimensions, 128 of 64) filled by TMA, one box per page, and four warps split a
 // stage by rows (groups of 16) and by positions, 32 at a time where they have them.
 // Each keeps its own running maximum and sum, joined at the end of the item. 64 single
-// tokens over 4.2 K positions of 32 heads of 128 (4.36 GB): 636 us, 105% of the copy
-// rate; 32 over 0.3 to 16 K positions of 8 heads: 170 us (90%); 64 over 1.1 K positions of
-// 12 heads of 64: 50 us (67%), 5 us of it before the first bytes are there.
+// tokens over 4.2 K positions of 32 heads of 128 (4.36 GB): 641 us, 104% of the copy
+// rate; 32 over 0.3 to 16 K positions of 8 heads: 173 us (89%); 64 over 1.1 K positions of
+// 12 heads of 64: 50 us (67%), with pages of 16 or 128 rows alike, 5 us of it before the
+// first bytes are there and 6 us the joining kernel.
 constexpr int SHORT_THREADS = 160, SHORT_LEAST = 2;  // (of 1, 2 and 4 units a part, 8 x 500 positions: 19, 13 and 13 us)
 
 template <int D>

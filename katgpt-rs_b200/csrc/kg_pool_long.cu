@@ -13,10 +13,11 @@
 // rows are exponentiated while the other tile's products run. (Two issuing threads let
 // the tiles fall into step, both waiting for the tensor pipe and then both for the
 // exponentials: 4640 cycles a pair of units at 1.70 GHz.)
-// 2048 tokens over 18000 positions, 32 query and 8 K/V heads of 128: 475 us cool, 535 to
-// 555 us under the power cap (1,030 to 1,200 TFLOP/s). A pair of units takes about 3,150
-// cycles, of which the products 2,055 and the exponentials 2,048 run beside each other:
-// bound by the chain scores -> exponentials -> values -> next scores of one tile.
+// 2048 tokens over 18000 positions, 32 query and 8 K/V heads of 128, bf16: 497 us between
+// pauses, 555 to 565 us back to back (1,010 to 1,030 TFLOP/s, under the power cap), f16 527;
+// heads of 64 455 us and 466. A pair of units takes about 3,150 cycles, of which the products
+// 2,055 and the exponentials 2,048 run beside each other: bound by the chain scores ->
+// exponentials -> values -> next scores of one tile.
 // A row's O is rescaled only when its maximum has grown by more than 2^LAG since the
 // last time: 2^8 in bf16, whose P then reaches at most 2^8; 2^3 in f16, whose P has to
 // use the range that it has (Cvt).
