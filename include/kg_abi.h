@@ -354,7 +354,8 @@ int kg_sample_logits_dev(kg_ctx *ctx, int32_t n_rows, int32_t vocab, int32_t dty
 
 /* Waits for the context's device and returns what the device-side checks of the
  * calls above saw since the last kg_pool_status: KG_OK, KG_ERR_INVALID_ARG or
- * KG_ERR_TIMEOUT. Not during a stream capture. */
+ * KG_ERR_TIMEOUT (a device-side wait ran out: the rows of a kg_pool_attend_dev call
+ * are undefined; it comes before rejected arguments). Not during a stream capture. */
 int kg_pool_status(kg_ctx *ctx);
 
 /* ---- multi-GPU sequence shards (one context per GPU) ----
