@@ -173,3 +173,20 @@ def test_large_scores_of_any_bits(kg, be, dt, rows):
             got, want, _ = _shared(kg, be, k, v, q, 1, dt, scale, 0)
             # the one probability is rounded and divided by itself unrounded, then the result: half a step each
             assert (np.abs(got - want) <= 2 * half * 1.01 * np.abs(want)).all(), (e, scale, np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,positions,d", [(1, 5000, 64), (3, 700, 128), (70, 5000, 128), (200, 1500, 64)])
+@pytest.mark.parametrize("span", [3.0, 30.0, -30.0, 300.0])
+def test_rising_and_falling_scores(kg, be, dt, rows, positions, d, span):
+    """The running maximum grows all the way, by little or by much in a unit, or is the first position's; rows differ in how
+    steeply."""
+    rng = np.random.default_rng(rows)
+    k, q = rng.standard_normal((positions, 2, d)) * 0.2, rng.standard_normal((rows, 4, d)) * 0.2
+    k[..., 0] = np.linspace(-0.5, 0.5, positions)[:, None] * span
+    q[..., 0] = d ** 0.5 * rng.uniform(0.1, 1.0, (rows, 4))
+    v = rng.standard_normal((positions, 2, d)) + 1.0
+    got, want, tol = _shared(kg, be, k, v, q, 2, dt, d ** -0.5, 1)
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+    again, _, _ = _shared(kg, be, k, v, q, 2, dt, d ** -0.5, 1)
+    np.testing.assert_array_equal(got, again)
